@@ -21,6 +21,23 @@ QOUT_MXFP8, QOUT_NVFP4 = 1, 2
 _c_i64 = ctypes.c_int64
 _c_vp = ctypes.c_void_p
 
+
+class Heads(ctypes.Structure):
+    """fp4t_heads_t: one [batch, tokens, heads, head_dim] tensor, strides in elements."""
+    _fields_ = [("data", _c_vp), ("heads", _c_i64), ("stride_batch", _c_i64), ("stride_token", _c_i64), ("stride_head", _c_i64)]
+
+
+class Rotary(ctypes.Structure):
+    """fp4t_rotary_t: positions and the table of turning pairs."""
+    _fields_ = [("positions", _c_vp), ("positions_i64", ctypes.c_int), ("stride_batch", _c_i64), ("stride_token", _c_i64),
+                ("stride_axis", _c_i64), ("axes", ctypes.c_int), ("turned", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("turns", _c_vp), ("axis", _c_vp)]
+
+
+_p_heads = ctypes.POINTER(Heads)
+_p_rotary = ctypes.POINTER(Rotary)
+_p_vps = ctypes.POINTER(_c_vp)
+
 _SIGNATURES = {
     "fp4t_last_error": (ctypes.c_char_p, []),
     "fp4t_version": (ctypes.c_int, []),
@@ -39,6 +56,13 @@ _SIGNATURES = {
     "fp4t_layernorm_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
     "fp4t_layernorm_backward": (ctypes.c_int, [_c_vp, ctypes.c_int, _c_i64, _c_vp, ctypes.c_int, _c_i64, _c_vp, _c_vp, _c_vp,
                                                 _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "fp4t_rotary": (ctypes.c_int, [_p_heads, _p_heads, ctypes.c_int, ctypes.c_int, _c_i64, _c_i64, _c_i64, _p_rotary, ctypes.c_int,
+                                   _c_vp]),
+    "fp4t_qk_norm_rotary_forward": (ctypes.c_int, [_p_heads, _p_vps, ctypes.c_float, _p_heads, ctypes.c_int, ctypes.c_int, _c_i64,
+                                                   _c_i64, _c_i64, _p_rotary, _c_vp]),
+    "fp4t_qk_norm_rotary_backward_workspace_bytes": (_c_i64, [_c_i64]),
+    "fp4t_qk_norm_rotary_backward": (ctypes.c_int, [_p_heads, _p_heads, _p_vps, ctypes.c_float, _p_heads, _p_vps, ctypes.c_int,
+                                                    ctypes.c_int, _c_i64, _c_i64, _c_i64, _p_rotary, _c_vp, _c_i64, _c_vp]),
     "fp4t_rank_meet": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                       ctypes.c_void_p, ctypes.c_void_p]),
     "fp4t_reduce_shard_bf16_multimem": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,

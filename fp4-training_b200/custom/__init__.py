@@ -10,6 +10,7 @@ from .linear.nvf4fwd_mxf8bwd import CublasltFwdNvfp4BwdMxfp8Linear
 from .linear.cuda_aten import AddmmLinear
 from .linear.fake_mxfp8 import FakeMxfp8Linear
 from .norm import FusedLayerNorm
+from .rotary import FusedQKNorm, RotaryPositions
 
 __all__ = [
     "CustomLinear",
@@ -20,4 +21,6 @@ __all__ = [
     "FakeMxfp8Linear",
     "AddmmLinear",
     "FusedLayerNorm",
+    "FusedQKNorm",
+    "RotaryPositions",
 ]

@@ -465,6 +465,62 @@ FP4T_API int fp4t_layernorm_backward(const void* dy, int dy_dtype, int64_t lddy,
                             int64_t rows, int64_t cols, void* dx, int64_t lddx, float* dgamma,
                             float* dbeta, void* workspace, fp4t_stream_t stream);
 
+/*
+ * Rotary positions with several axes, and the per-head RMS norm of queries and keys with that
+ * rotation in the same pass.  They stand between the stacked q / k / v projection and the attention
+ * core; the reference has neither (its blocks take positions from a learned embedding,
+ * models/vit.py:50-56, and use q and k as projected, models/transformer_block.py:89-95).
+ *
+ * A tensor of heads is [batch, tokens, heads, head_dim] with unit stride in the last dimension and
+ * the other strides given in elements, so views of the stacked projection's output and [batch, heads,
+ * tokens, head_dim] tensors are taken as they are.  Each call takes one or two such tensors (queries
+ * and keys, which may have different numbers of heads) of one dtype (FP4T_DT_*); y may be x.
+ * head_dim is even, at most 512.  Host structures; the pointers in them are device pointers.
+ */
+typedef struct {
+  void* data;
+  int64_t heads, stride_batch, stride_token, stride_head;
+} fp4t_heads_t;
+
+/*
+ * Which pairs of a head turn, and how far.  `turned` pairs (0: none, at most head_dim / 2) turn, the
+ * elements behind them are copied: pair p is elements (p, p + turned), or (2p, 2p + 1) if `interleaved`.
+ * Its angle is positions[b, l, axis[p]] * turns[p] * 2^-64 turns modulo one turn, exact to 2^-32
+ * turns for every 64-bit position (negative ones too).  turns, axis: [turned] on the device;
+ * an axis value outside [0, axes) is read as the last axis.  positions: int64
+ * (positions_i64 = 1) or int32 with strides in elements (0 for a dimension that is shared).
+ */
+typedef struct {
+  const void* positions;
+  int positions_i64;
+  int64_t stride_batch, stride_token, stride_axis;
+  int axes, turned, interleaved;
+  const uint64_t* turns;
+  const int32_t* axis;
+} fp4t_rotary_t;
+
+/* y = R(+-angle) x (inverse = 1: the other direction, which is the backward pass). */
+FP4T_API int fp4t_rotary(const fp4t_heads_t* x, const fp4t_heads_t* y, int count, int dtype, int64_t batch,
+                         int64_t tokens, int64_t head_dim, const fp4t_rotary_t* rotary, int inverse,
+                         fp4t_stream_t stream);
+/*
+ * forward:  y = R(angle) (w * x / sqrt(mean(x^2) + eps)), the mean over a head's head_dim elements in
+ *   fp32; weights[i]: fp32 [head_dim] of tensor i, 16-byte aligned.
+ * backward: dx and dweights[i] (fp32 [head_dim]) from dy and x; nothing but x is kept by the forward
+ *   pass.  workspace: 16-byte aligned, fp4t_qk_norm_rotary_backward_workspace_bytes(head_dim) bytes (less
+ *   makes the call slower); the weight gradients are added in a fixed order (reproducible).
+ */
+FP4T_API int fp4t_qk_norm_rotary_forward(const fp4t_heads_t* x, const float* const* weights, float eps,
+                                         const fp4t_heads_t* y, int count, int dtype, int64_t batch,
+                                         int64_t tokens, int64_t head_dim, const fp4t_rotary_t* rotary,
+                                         fp4t_stream_t stream);
+FP4T_API int64_t fp4t_qk_norm_rotary_backward_workspace_bytes(int64_t head_dim);
+FP4T_API int fp4t_qk_norm_rotary_backward(const fp4t_heads_t* dy, const fp4t_heads_t* x,
+                                          const float* const* weights, float eps, const fp4t_heads_t* dx,
+                                          float* const* dweights, int count, int dtype, int64_t batch,
+                                          int64_t tokens, int64_t head_dim, const fp4t_rotary_t* rotary,
+                                          void* workspace, int64_t workspace_bytes, fp4t_stream_t stream);
+
 /* Byte-matrix transpose [rows, cols] -> [cols, rows] (E4M3 codes for the NN / NT operand
  * forms of custom/backend/csrc/cublaslt_mm_mxfp8.cu:70-88). */
 FP4T_API int fp4t_transpose_bytes(const void* src, void* dst, int64_t rows, int64_t cols,

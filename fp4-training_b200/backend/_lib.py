@@ -17,6 +17,8 @@ LIB_PATH = os.path.join(_HERE, "..", "lib", "libfp4t.so")
 DT_BF16, DT_F32 = 0, 1
 SR_NONE, SR_NOISE, SR_HASH = 0, 1, 2
 QOUT_MXFP8, QOUT_NVFP4 = 1, 2
+XENT_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+STATUS_BAD_TARGET = 41
 
 _c_i64 = ctypes.c_int64
 _c_vp = ctypes.c_void_p
@@ -63,6 +65,13 @@ _SIGNATURES = {
     "fp4t_qk_norm_rotary_backward_workspace_bytes": (_c_i64, [_c_i64]),
     "fp4t_qk_norm_rotary_backward": (ctypes.c_int, [_p_heads, _p_heads, _p_vps, ctypes.c_float, _p_heads, _p_vps, ctypes.c_int,
                                                     ctypes.c_int, _c_i64, _c_i64, _c_i64, _p_rotary, _c_vp, _c_i64, _c_vp]),
+    "fp4t_linear_xent_forward_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "fp4t_linear_xent_forward": (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_int, _c_vp, _c_i64, _c_i64, _c_i64,
+                                                _c_i64, ctypes.c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp]),
+    "fp4t_linear_xent_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int]),
+    "fp4t_linear_xent_backward": (ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_int, _c_vp, _c_vp, _c_vp,
+                                                 _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_vp, ctypes.c_int, _c_vp,
+                                                 ctypes.c_int, _c_vp, ctypes.c_int, _c_vp, _c_i64, _c_vp, _c_vp]),
     "fp4t_rank_meet": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                       ctypes.c_void_p, ctypes.c_void_p]),
     "fp4t_reduce_shard_bf16_multimem": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,

@@ -63,6 +63,8 @@ def check_status(device="cuda") -> None:
         # a kernel that gave up may have left its tile counters nonzero
         with torch.cuda.device(s.device):
             _lib.check(_lib.lib().fp4t_reset_tile_counters(_lib.stream_ptr(s.device)), "fp4t_reset_tile_counters")
+        if code == _lib.STATUS_BAD_TARGET:
+            raise RuntimeError("a cross-entropy target lies outside the vocabulary (its token's loss is NaN)")
         raise RuntimeError(f"fp4t kernel abandoned a wait (role code {code})")
 
 
@@ -670,3 +672,100 @@ def qk_norm_rotary_backward(dy, x, weights, eps, positions=None, table=None):
         _lib.check(rc, "fp4t_qk_norm_rotary_backward")
         LAUNCHES["rotary"] += 2
     return dx, dw
+
+
+# ------------------------------------------------------------------ linear cross entropy
+def _xent_rows(t, name):
+    """2-D bf16 tensor with rows the kernels can load: unit column stride, 16-byte aligned rows."""
+    _need_cuda(t)
+    if t.ndim != 2 or t.dtype != torch.bfloat16:
+        raise ValueError(f"linear_cross_entropy: {name} must be a 2-D bfloat16 tensor")
+    rows, dim = t.shape
+    if t.stride(1) != 1 or t.data_ptr() % 16 or (rows > 1 and (t.stride(0) % 8 or t.stride(0) < dim)):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t, (t.stride(0) if rows > 1 else dim)
+
+
+def _xent_args(h, w, bias, target, reduction):
+    h, ldh = _xent_rows(h, "hidden")
+    w, ldw = _xent_rows(w, "weight")
+    _need_cuda(target, bias)
+    if h.shape[1] != w.shape[1]:
+        raise ValueError(f"linear_cross_entropy: hidden is {h.shape[1]} wide, weight {w.shape[1]}")
+    if h.shape[1] % 8 or h.shape[1] == 0:
+        raise ValueError(f"linear_cross_entropy needs a width that is a multiple of 8, got {h.shape[1]}")
+    if w.shape[0] == 0:
+        raise ValueError("linear_cross_entropy: the vocabulary is empty")
+    if target.shape != (h.shape[0],) or target.dtype != torch.int64:
+        raise ValueError(f"linear_cross_entropy: target must be int64 [{h.shape[0]}]")
+    if reduction not in _lib.XENT_REDUCTION:
+        raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    if bias is not None:
+        if bias.shape != (w.shape[0],) or bias.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"linear_cross_entropy: bias must be float32 or bfloat16 [{w.shape[0]}]")
+        bias = bias.contiguous()
+        if bias.data_ptr() % 16:
+            bias = bias.clone()
+    for t in (w, target, bias):
+        if t is not None and t.device != h.device:
+            raise ValueError("linear_cross_entropy: all tensors must be on one device")
+    return h, ldh, w, ldw, bias, target.contiguous()
+
+
+def linear_cross_entropy_forward(h, w, bias, target, ignore_index=-100, reduction="mean"):
+    """Cross entropy of h @ w.T + bias without the logits.  h [T, D], w [V, D] bf16, bias [V] fp32 / bf16 or
+    None, target [T] int64 -> (loss [] or, reduction "none", [T]; lse [T]; count []), all fp32."""
+    h, ldh, w, ldw, bias, target = _xent_args(h, w, bias, target, reduction)
+    dev, (T, D), V = h.device, h.shape, w.shape[0]
+    with _on_device(dev):
+        stats = torch.empty(T + 1, dtype=torch.float32, device=dev)
+        lse, count = stats[:T], stats[T]
+        if T == 0:
+            count.zero_()
+            empty = {"none": 0, "sum": 1, "mean": 1}[reduction]
+            return torch.full((empty,) if not empty else (), float("nan") if reduction == "mean" else 0.0, device=dev), lse, count
+        loss = torch.empty(T if reduction == "none" else (), dtype=torch.float32, device=dev)
+        L = _lib.lib()
+        ws_bytes = L.fp4t_linear_xent_forward_workspace_bytes(T, V)
+        if ws_bytes < 0:
+            _lib.check(-1, "fp4t_linear_xent_forward_workspace_bytes")
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        rc = L.fp4t_linear_xent_forward(h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias),
+                                        0 if bias is None else _lib.dtype_code(bias.dtype), target.data_ptr(), T, D, V,
+                                        int(ignore_index), _lib.XENT_REDUCTION[reduction], loss.data_ptr(), lse.data_ptr(),
+                                        count.data_ptr(), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+        _lib.check(rc, "fp4t_linear_xent_forward")
+        LAUNCHES["xent"] += 2 * (-(-T // 16384))
+    return loss, lse, count
+
+
+def linear_cross_entropy_backward(grad_loss, h, w, bias, target, lse, count, ignore_index=-100, reduction="mean",
+                                  dh_dtype=None, dw_dtype=None, db_dtype=None):
+    """-> (dh [T, D], dw [V, D], db [V]) in the dtypes asked for (None: not computed) for the forward above."""
+    h, ldh, w, ldw, bias, target = _xent_args(h, w, bias, target, reduction)
+    dev, (T, D), V = h.device, h.shape, w.shape[0]
+    _need_cuda(grad_loss, lse, count)
+    grad_loss = grad_loss.to(torch.float32).contiguous()
+    if grad_loss.numel() != (T if reduction == "none" else 1):
+        raise ValueError("linear_cross_entropy: grad_loss must have the shape of the loss")
+    with _on_device(dev):
+        make = lambda shape, dt: None if dt is None else (torch.zeros if T == 0 else torch.empty)(shape, dtype=dt, device=dev)  # noqa: E731
+        dh, dw, db = make((T, D), dh_dtype), make((V, D), dw_dtype), make((V,), db_dtype)
+        if T == 0 or (dh is None and dw is None and db is None):
+            return dh, dw, db
+        L = _lib.lib()
+        ws_bytes = L.fp4t_linear_xent_backward_workspace_bytes(T, D, V, int(dh is not None), int(dw is not None))
+        if ws_bytes < 0:
+            raise RuntimeError("fp4t_linear_xent_backward_workspace_bytes: unsupported shape or device")
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        code = lambda t: 0 if t is None else _lib.dtype_code(t.dtype)  # noqa: E731
+        rc = L.fp4t_linear_xent_backward(grad_loss.data_ptr(), h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias), code(bias),
+                                         target.data_ptr(), lse.data_ptr(), count.data_ptr(), T, D, V, int(ignore_index),
+                                         _lib.XENT_REDUCTION[reduction], _lib.ptr(dh), code(dh), _lib.ptr(dw), code(dw),
+                                         _lib.ptr(db), code(db), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(),
+                                         _lib.stream_ptr(dev))
+        _lib.check(rc, "fp4t_linear_xent_backward")
+        LAUNCHES["xent"] += 1 + int(dh is not None) + int(dw is not None) + int(db is not None)
+    return dh, dw, db

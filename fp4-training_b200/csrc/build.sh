@@ -10,7 +10,7 @@ ARCH=(-gencode arch=compute_100a,code=sm_100a)
 tmp="$(mktemp -d)"
 trap 'rm -rf "$tmp"' EXIT
 pids=()
-for unit in quantize gemm misc linear allreduce norm rotary; do
+for unit in quantize gemm misc linear allreduce norm rotary xent; do
   "$NVCC" "${ARCH[@]}" -O3 -lineinfo -std=c++17 -Xcompiler -fPIC -Xcompiler -fvisibility=hidden ${FP4T_NVCC_EXTRA:-} \
     -c -o "$tmp/$unit.o" "$here/fp4t_$unit.cu" &
   pids+=($!)

@@ -227,6 +227,7 @@ extern "C" int fp4t_set_wait_timeout_ns(uint64_t ns) {
   int rc = fp4t::set_wait_timeout_gemm(ns);
   if (rc == FP4T_OK) rc = fp4t::set_wait_timeout_quantize(ns);
   if (rc == FP4T_OK) rc = fp4t::set_wait_timeout_allreduce(ns);
+  if (rc == FP4T_OK) rc = fp4t::set_wait_timeout_xent(ns);
   return rc;
 }
 

@@ -9,6 +9,7 @@ from .linear.nvf4fwd_mxf8bwd import CublasltFwdNvfp4BwdMxfp8Linear
 
 from .linear.cuda_aten import AddmmLinear
 from .linear.fake_mxfp8 import FakeMxfp8Linear
+from .loss import LinearCrossEntropy, linear_cross_entropy
 from .norm import FusedLayerNorm
 from .rotary import FusedQKNorm, RotaryPositions
 
@@ -22,5 +23,7 @@ __all__ = [
     "AddmmLinear",
     "FusedLayerNorm",
     "FusedQKNorm",
+    "LinearCrossEntropy",
     "RotaryPositions",
+    "linear_cross_entropy",
 ]

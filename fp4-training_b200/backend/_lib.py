@@ -65,11 +65,11 @@ _SIGNATURES = {
     "fp4t_qk_norm_rotary_backward_workspace_bytes": (_c_i64, [_c_i64]),
     "fp4t_qk_norm_rotary_backward": (ctypes.c_int, [_p_heads, _p_heads, _p_vps, ctypes.c_float, _p_heads, _p_vps, ctypes.c_int,
                                                     ctypes.c_int, _c_i64, _c_i64, _c_i64, _p_rotary, _c_vp, _c_i64, _c_vp]),
-    "fp4t_linear_xent_forward_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "fp4t_linear_xent_forward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
     "fp4t_linear_xent_forward": (ctypes.c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_int, _c_vp, _c_i64, _c_i64, _c_i64,
                                                 _c_i64, ctypes.c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp]),
-    "fp4t_linear_xent_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int]),
-    "fp4t_linear_xent_backward": (ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_int, _c_vp, _c_vp, _c_vp,
+    "fp4t_linear_xent_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "fp4t_linear_xent_backward": (ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, ctypes.c_int, _c_vp, _c_vp,
                                                  _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_vp, ctypes.c_int, _c_vp,
                                                  ctypes.c_int, _c_vp, ctypes.c_int, _c_vp, _c_i64, _c_vp, _c_vp]),
     "fp4t_rank_meet": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int, ctypes.c_int,

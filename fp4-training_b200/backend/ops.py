@@ -716,7 +716,8 @@ def _xent_args(h, w, bias, target, reduction):
 
 def linear_cross_entropy_forward(h, w, bias, target, ignore_index=-100, reduction="mean"):
     """Cross entropy of h @ w.T + bias without the logits.  h [T, D], w [V, D] bf16, bias [V] fp32 / bf16 or
-    None, target [T] int64 -> (loss [] or, reduction "none", [T]; lse [T]; count []), all fp32."""
+    None, target [T] int64 -> (loss [] or, reduction "none", [T]; lse [T],
+    of the counted tokens in order; count []), all fp32."""
     h, ldh, w, ldw, bias, target = _xent_args(h, w, bias, target, reduction)
     dev, (T, D), V = h.device, h.shape, w.shape[0]
     with _on_device(dev):
@@ -728,7 +729,7 @@ def linear_cross_entropy_forward(h, w, bias, target, ignore_index=-100, reductio
             return torch.full((empty,) if not empty else (), float("nan") if reduction == "mean" else 0.0, device=dev), lse, count
         loss = torch.empty(T if reduction == "none" else (), dtype=torch.float32, device=dev)
         L = _lib.lib()
-        ws_bytes = L.fp4t_linear_xent_forward_workspace_bytes(T, V)
+        ws_bytes = L.fp4t_linear_xent_forward_workspace_bytes(T, D, V)
         if ws_bytes < 0:
             _lib.check(-1, "fp4t_linear_xent_forward_workspace_bytes")
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
@@ -737,16 +738,16 @@ def linear_cross_entropy_forward(h, w, bias, target, ignore_index=-100, reductio
                                         int(ignore_index), _lib.XENT_REDUCTION[reduction], loss.data_ptr(), lse.data_ptr(),
                                         count.data_ptr(), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(), _lib.stream_ptr(dev))
         _lib.check(rc, "fp4t_linear_xent_forward")
-        LAUNCHES["xent"] += 2 * (-(-T // 16384))
+        LAUNCHES["xent"] += 1 + 2 * (-(-T // 16384))
     return loss, lse, count
 
 
-def linear_cross_entropy_backward(grad_loss, h, w, bias, target, lse, count, ignore_index=-100, reduction="mean",
+def linear_cross_entropy_backward(grad_loss, h, w, bias, target, lse, ignore_index=-100, reduction="mean",
                                   dh_dtype=None, dw_dtype=None, db_dtype=None):
     """-> (dh [T, D], dw [V, D], db [V]) in the dtypes asked for (None: not computed) for the forward above."""
     h, ldh, w, ldw, bias, target = _xent_args(h, w, bias, target, reduction)
     dev, (T, D), V = h.device, h.shape, w.shape[0]
-    _need_cuda(grad_loss, lse, count)
+    _need_cuda(grad_loss, lse)
     grad_loss = grad_loss.to(torch.float32).contiguous()
     if grad_loss.numel() != (T if reduction == "none" else 1):
         raise ValueError("linear_cross_entropy: grad_loss must have the shape of the loss")
@@ -756,16 +757,16 @@ def linear_cross_entropy_backward(grad_loss, h, w, bias, target, lse, count, ign
         if T == 0 or (dh is None and dw is None and db is None):
             return dh, dw, db
         L = _lib.lib()
-        ws_bytes = L.fp4t_linear_xent_backward_workspace_bytes(T, D, V, int(dh is not None), int(dw is not None))
+        ws_bytes = L.fp4t_linear_xent_backward_workspace_bytes(T, D, V, int(dh is not None), int(dw is not None), int(db is not None))
         if ws_bytes < 0:
             raise RuntimeError("fp4t_linear_xent_backward_workspace_bytes: unsupported shape or device")
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         code = lambda t: 0 if t is None else _lib.dtype_code(t.dtype)  # noqa: E731
         rc = L.fp4t_linear_xent_backward(grad_loss.data_ptr(), h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias), code(bias),
-                                         target.data_ptr(), lse.data_ptr(), count.data_ptr(), T, D, V, int(ignore_index),
+                                         target.data_ptr(), lse.data_ptr(), T, D, V, int(ignore_index),
                                          _lib.XENT_REDUCTION[reduction], _lib.ptr(dh), code(dh), _lib.ptr(dw), code(dw),
                                          _lib.ptr(db), code(db), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(),
                                          _lib.stream_ptr(dev))
         _lib.check(rc, "fp4t_linear_xent_backward")
-        LAUNCHES["xent"] += 1 + int(dh is not None) + int(dw is not None) + int(db is not None)
+        LAUNCHES["xent"] += 2 + int(dh is not None) + int(dw is not None) + int(db is not None)
     return dh, dw, db

@@ -51,24 +51,31 @@ constexpr int64_t kTokenBlock = 16384;           // tokens whose partial statist
 constexpr int64_t kPieceBytes = 512ll << 20;     // dl of one piece of the vocabulary, unless that makes
 constexpr int64_t kMinPiece = 4096;              // the piece narrower than this
 
+// Counted tokens are numbered in order ("slots"); everything between the operands and the gradients has
+// slots for rows.  Their number is known on the device only.
 struct XParams {
-  int rows, cols;                                // of the output
+  int rows, cols;                                // of the output; rows: the most there can be
   int m_tiles, n_tiles, group_m, k_stages, splits, ks_per_split, slice_rows;
+  const int* slots;                              // number of counted tokens
+  int tokens;                                    // all tokens: slots == tokens means that h can be read as it is
+  int slot0;                                     // kStats: first slot of the block
   // kStats, kGrad
   const void* bias;
   int bias_f32;
-  const int64_t* target;
-  int64_t ignore;
-  int64_t col0;                                  // first vocabulary entry of the piece
+  const int* target;                             // of the slots; -1: outside the vocabulary
+  int col0;                                      // first vocabulary entry of the piece
   float2* part;                                  // kStats: [2 * n_tiles][rows] (maximum, sum)
   float* picked;                                 // kStats: the target's logit
-  unsigned int* counter;                         // kStats: put to zero for the joining kernel
   const float* lse;
   const float* grad;
   int grad_per_row;
-  const float* count;                            // kGrad, mean: number of counted tokens
+  int mean;                                      // kGrad: divide by the number of counted tokens
+  const int* token;                              // slot -> token (grad_per_row, and kProduct's rows)
+  float* col_part;                               // kGrad: column sums of dl over 32 slots, [slots / 32][col_ld], or null
+  int64_t col_ld;
   // kProduct, kProductT
   int out_f32;
+  void* out;                                     // kProduct: the result's rows are tokens, not slots, if not null
   const float* acc;                              // added to the result (fp32, pitch ldacc)
   int64_t ldacc;
   int32_t* status;
@@ -168,6 +175,24 @@ __device__ __forceinline__ void add_bias(const XParams& g, int c, float (&v)[32]
   }
 }
 
+// Sums over the warp's 32 rows of 32 columns, column j's in lane j: in each step a lane hands half of its
+// columns to the lane across and adds what it gets for the other half, 31 shuffles in all.
+__device__ __forceinline__ float column_sums(const float (&v)[32], int lane) {
+  float w[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) w[j] = v[j];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool upper = (lane & o) != 0;
+#pragma unroll
+    for (int j = 0; j < o; ++j) {
+      const float give = upper ? w[j] : w[j + o], keep = upper ? w[j + o] : w[j];
+      w[j] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+    }
+  }
+  return w[0];
+}
+
 // One 32 x 32 chunk (a row per lane) to a swizzled staging tile and from there with one tiled TMA
 // store, clipped at the matrix edges.  bf16: two 2-KB tiles that alternate; fp32: one of 4 KB.
 __device__ __forceinline__ void store_chunk_bf16(const CUtensorMap* map, uint8_t* buf, uint32_t& n_emit, int lane, int row, int col,
@@ -207,11 +232,35 @@ __device__ __forceinline__ void store_chunk_f32(const CUtensorMap* map, uint8_t*
   }
 }
 
+// The same chunk to rows that are not neighbours: each lane its own (columns are a multiple of 8).
+__device__ __forceinline__ void store_row_chunk(void* row, int out_f32, int col, int cols, const float (&v)[32]) {
+  if (row == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (col + 8 * j < cols) {
+      if (out_f32) {
+        float4* p = reinterpret_cast<float4*>(static_cast<float*>(row) + col + 8 * j);
+        p[0] = make_float4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
+        p[1] = make_float4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * t], v[8 * j + 2 * t + 1]);
+          w[t] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(row) + col + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+
 template <int kMode, int kBN>
 __global__ void __launch_bounds__(kXThreads, 1)
 xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                 const __grid_constant__ CUtensorMap map_d, const XParams g) {
+                 const __grid_constant__ CUtensorMap map_packed, const __grid_constant__ CUtensorMap map_d, const XParams gp) {
   using C = XCfg<kBN>;
+  XParams g = gp;
   constexpr bool kAMn = kMode == kProductT, kBMn = kMode == kProduct || kMode == kProductT;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t smem_base = smem_u32(smem);
@@ -237,6 +286,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   if (threadIdx.x == 32) {
     tma_prefetch_map(&map_a);
     tma_prefetch_map(&map_b);
+    if (kMode != kProduct) tma_prefetch_map(&map_packed);
     if (kMode != kStats) tma_prefetch_map(&map_d);
   }
   if (threadIdx.x == 0) {
@@ -263,6 +313,18 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();                  // from here on memory that the predecessor wrote is touched
 
+  // The work follows the number of counted tokens: rows of the output, or the length of K.
+  const int slots = *static_cast<const volatile int*>(g.slots);
+  const bool dense = slots == g.tokens;
+  if (kMode == kProductT) {
+    g.k_stages = (slots + kXK - 1) / kXK;
+    g.ks_per_split = (g.k_stages + g.splits - 1) / g.splits;
+  } else {
+    g.rows = max(0, min(g.rows, slots - g.slot0));
+    g.m_tiles = (g.rows + kXM - 1) / kXM;
+  }
+  const CUtensorMap* tma_a = (kMode == kStats || kMode == kGrad) && !dense ? &map_packed : &map_a;
+  const CUtensorMap* tma_b = kMode == kProductT && !dense ? &map_packed : &map_b;
   const int units = g.m_tiles * g.n_tiles * g.splits;
   const uint32_t leader_full = mapa_u32(bar_full, 0);
   const uint32_t leader_tmem_empty = mapa_u32(bar_tmem_empty, 0);
@@ -283,16 +345,16 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           const uint32_t bar = leader_full + 8 * stage;
           if (leader) mbar_expect_tx(bar_full + 8 * stage, 2u * C::kStageBytes);
           if (kAMn) {
-            tma_load_2d_pair(a_s, &map_a, bar, row_a, ks * kXK);
-            tma_load_2d_pair(a_s + 8192, &map_a, bar, row_a + 64, ks * kXK);
+            tma_load_2d_pair(a_s, tma_a, bar, row_a, ks * kXK);
+            tma_load_2d_pair(a_s + 8192, tma_a, bar, row_a + 64, ks * kXK);
           } else {
-            tma_load_2d_pair(a_s, &map_a, bar, ks * kXK, row_a);
+            tma_load_2d_pair(a_s, tma_a, bar, ks * kXK, row_a);
           }
           if (kBMn) {
 #pragma unroll
-            for (int o = 0; o < C::kBRows / 64; ++o) tma_load_2d_pair(b_s + o * 8192, &map_b, bar, row_b + o * 64, ks * kXK);
+            for (int o = 0; o < C::kBRows / 64; ++o) tma_load_2d_pair(b_s + o * 8192, tma_b, bar, row_b + o * 64, ks * kXK);
           } else {
-            tma_load_2d_pair(b_s, &map_b, bar, ks * kXK, row_b);
+            tma_load_2d_pair(b_s, tma_b, bar, ks * kXK, row_b);
           }
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
@@ -348,8 +410,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     uint8_t* buf = smem + C::kEpi0 + (warp - 4) * 4096;
     uint32_t n_emit = 0;
     float scale = 0.f;
-    if (kMode == kStats && blockIdx.x == 0 && threadIdx.x == 128) *g.counter = 0u;
-    if (kMode == kGrad && !g.grad_per_row) scale = g.count != nullptr ? __ldg(g.grad) / __ldg(g.count) : __ldg(g.grad);
+    if (kMode == kGrad && !g.grad_per_row) scale = g.mean ? __ldg(g.grad) / (float)slots : __ldg(g.grad);
     int it = 0;
     for (int unit = cluster_id; unit < units; unit += num_clusters, ++it) {
       const TilePos t = tile_at(g, unit);
@@ -369,16 +430,16 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (lane == 0) mbar_arrive_cluster(leader_tmem_empty + 8 * a);
       };
       if (kMode == kStats || kMode == kGrad) {
-        const int64_t y = row_ok ? __ldg(reinterpret_cast<const long long*>(g.target) + row) : g.ignore;
-        const bool counted = y != g.ignore;
         // the target's column in this warp's part of the tile; anything outside [0, cols) never matches
-        const int64_t yc = y - g.col0;
-        const int mine = counted && yc >= colbase && yc < colbase + C::kHalf && yc < g.cols ? (int)yc - colbase : -1;
+        const int yc = row_ok ? __ldg(g.target + row) - g.col0 : -1;
+        const int mine = yc >= colbase && yc < colbase + C::kHalf && yc < g.cols ? yc - colbase : -1;
+        // dl's rows up to the end of the last K stage that reads them are written (as zeros)
+        const int row_end = kMode == kGrad ? (g.rows + kXK - 1) / kXK * kXK : g.rows;
         float m = -INFINITY, s = 0.f, x_y = 0.f;
         float lse = 0.f, gr = 0.f;
         if (kMode == kGrad) {
           lse = row_ok ? __ldg(g.lse + row) : 0.f;
-          gr = g.grad_per_row ? (row_ok ? __ldg(g.grad + row) : 0.f) : scale;
+          gr = g.grad_per_row ? (row_ok ? __ldg(g.grad + __ldg(g.token + row)) : 0.f) : scale;
         }
 #pragma unroll 1
         for (int c = 0; c < C::kHalf / 32; ++c) {
@@ -387,7 +448,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           tc_wait_ld();
           if (c == C::kHalf / 32 - 1) release();
           const int col = colbase + c * 32;
-          if (col >= g.cols || row0 >= g.rows) continue;      // warp-uniform
+          if (col >= g.cols || row0 >= row_end) continue;     // warp-uniform
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -441,15 +502,23 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (mine == c * 32 + j) v[j] -= 1.f;
             }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = counted ? v[j] * gr : 0.f;
+            for (int j = 0; j < 32; ++j) v[j] = row_ok ? v[j] * gr : 0.f;
+            if (g.col_part != nullptr) {
+              const float sum = column_sums(v, lane);
+              if (col + lane < g.cols) g.col_part[(int64_t)(row0 >> 5) * g.col_ld + col + lane] = sum;
+            }
             store_chunk_bf16(&map_d, buf, n_emit, lane, row0, col, v);
           }
         }
         if (kMode == kStats && row_ok) {
-          g.part[(int64_t)(2 * t.n + half) * g.rows + row] = make_float2(m, s);
+          g.part[(int64_t)(2 * t.n + half) * gp.rows + row] = make_float2(m, s);
           if (mine >= 0) g.picked[row] = x_y;
         }
       } else {
+        const bool nothing = t.split * g.ks_per_split >= g.k_stages;    // no stage of K: no product was issued
+        void* out_row = nullptr;
+        if (kMode == kProduct && g.out != nullptr && !dense && row_ok)
+          out_row = static_cast<uint8_t*>(g.out) + (int64_t)__ldg(g.token + row) * g.cols * (g.out_f32 ? 4 : 2);
 #pragma unroll 1
         for (int c = 0; c < C::kHalf / 32; ++c) {
           uint32_t r[32];
@@ -460,7 +529,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           if (col >= g.cols || row0 >= g.rows) continue;
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          for (int j = 0; j < 32; ++j) v[j] = nothing ? 0.f : __uint_as_float(r[j]);
           if (g.acc != nullptr && row_ok) {                    // columns are a multiple of 8: whole vectors
             const float4* p = reinterpret_cast<const float4*>(g.acc + (int64_t)row * g.ldacc + col);
 #pragma unroll
@@ -472,7 +541,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
           }
           const int srow = row0 + t.split * g.slice_rows;
-          if (g.out_f32) store_chunk_f32(&map_d, buf, lane, srow, col, v);
+          if (kMode == kProduct && g.out != nullptr && !dense) store_row_chunk(out_row, g.out_f32, col, g.cols, v);
+          else if (g.out_f32) store_chunk_f32(&map_d, buf, lane, srow, col, v);
           else store_chunk_bf16(&map_d, buf, n_emit, lane, srow, col, v);
         }
       }
@@ -491,7 +561,130 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   }
 }
 
-// Joins the partial statistics of a row along the vocabulary: `lanes` rows a block (a power of two, at
+// Numbers the counted tokens in order and, unless all are counted, copies their rows of h together, so
+// that padded and masked-out tokens (a third to nine tenths of a fine-tuning batch) cost no products and their
+// contents reach nothing.  Each block takes a run of tokens; the counted ones before it are counted by
+// the block itself (64 KB of targets at 8192 tokens), for long inputs from per-run counts.
+constexpr int kPackThreads = 256;
+constexpr int64_t kPackSelf = 32768;             // tokens up to which every block counts for itself
+struct PackParams {
+  const int64_t* target;
+  int64_t ignore;
+  int vocab, tokens, run;                        // run: tokens per block
+  const int* run_counts;                         // counted tokens of every run, or null
+  const __nv_bfloat16* h;
+  int64_t ldh;
+  int dim;
+  __nv_bfloat16* packed;                         // [tokens][dim]
+  int* slots;
+  int* token;                                    // slot -> token
+  int* slot_target;
+  float* row_loss;                               // forward, losses token by token: 0 for the others
+  void* dh;                                      // backward: rows of the others are zero
+  int dh_f32;
+  unsigned int* counter;                         // forward: put to zero for the joining kernel
+  float* count;                                  // forward: number of counted tokens for the caller
+};
+__device__ __forceinline__ int pack_block_sum(int v, int* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = __reduce_add_sync(0xFFFFFFFFu, v);
+  __syncthreads();
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < kPackThreads / 32; ++w) s += red[w];
+  return s;
+}
+__global__ void __launch_bounds__(kPackThreads) xent_run_count_kernel(const int64_t* target, int64_t ignore, int tokens, int run, int* run_counts) {
+  __shared__ int red[kPackThreads / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t t0 = (int64_t)blockIdx.x * run, t1 = min((int64_t)tokens, t0 + run);
+  int n = 0;
+  for (int64_t t = t0 + threadIdx.x; t < t1; t += kPackThreads) n += target[t] != ignore;
+  n = pack_block_sum(n, red);
+  if (threadIdx.x == 0) run_counts[blockIdx.x] = n;
+}
+__global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParams p) {
+  __shared__ int red[kPackThreads / 32];
+  __shared__ int source[kPackThreads];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * p.run, t1 = min(p.tokens, t0 + p.run);      // gridDim * run < 2^31
+  int before = 0, all = 0;
+  if (p.run_counts != nullptr) {
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += kPackThreads) {
+      const int c = p.run_counts[i];
+      all += c;
+      if (i < (int)blockIdx.x) before += c;
+    }
+  } else {
+    for (int t = threadIdx.x; t < p.tokens; t += kPackThreads) {
+      const int c = __ldg(reinterpret_cast<const long long*>(p.target) + t) != p.ignore;
+      all += c;
+      if (t < t0) before += c;
+    }
+  }
+  all = pack_block_sum(all, red);
+  before = pack_block_sum(before, red);
+  const bool dense = all == p.tokens;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *p.slots = all;
+    if (p.counter) *p.counter = 0u;
+    if (p.count) *p.count = (float)all;
+  }
+  for (int base = t0; base < t1; base += kPackThreads) {
+    const int t = base + (int)threadIdx.x;
+    const int64_t y = t < t1 ? __ldg(reinterpret_cast<const long long*>(p.target) + t) : p.ignore;
+    const bool counted = t < t1 && y != p.ignore;
+    const uint32_t votes = __ballot_sync(0xFFFFFFFFu, counted);
+    __syncthreads();                              // red and source of the round before are read
+    if (lane == 0) red[warp] = __popc(votes);
+    __syncthreads();
+    int at = __popc(votes & ((1u << lane) - 1u)), total = 0;
+#pragma unroll
+    for (int w = 0; w < kPackThreads / 32; ++w) {
+      if (w < warp) at += red[w];
+      total += red[w];
+    }
+    if (counted) {
+      p.token[before + at] = t;
+      p.slot_target[before + at] = y >= 0 && y < p.vocab ? (int)y : -1;
+      source[at] = t;
+    } else if (t < t1 && p.row_loss != nullptr) {
+      p.row_loss[t] = 0.f;
+    }
+    __syncthreads();
+    if (!dense) {
+      for (int i = warp; i < total; i += kPackThreads / 32) {
+        const uint4* from = reinterpret_cast<const uint4*>(p.h + (int64_t)source[i] * p.ldh);
+        uint4* to = reinterpret_cast<uint4*>(p.packed + (int64_t)(before + i) * p.dim);
+        for (int c = lane; c < p.dim / 8; c += 32) to[c] = from[c];
+      }
+      if (p.dh != nullptr) {
+        const int vecs = p.dim / (p.dh_f32 ? 4 : 8);
+        for (int i = 0; i < 32; ++i) {            // a warp its own 32 tokens
+          const int tt = base + warp * 32 + i;
+          if (tt < t1 && !((votes >> i) & 1u)) {
+            uint4* to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.dh) + (int64_t)tt * vecs * 16);
+            for (int c = lane; c < vecs; c += 32) to[c] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+      }
+    }
+    before += total;
+  }
+  // the rows behind the last slot that the last K stage of dW reads are zero
+  if (!dense && blockIdx.x == gridDim.x - 1) {
+    const int end = min(p.tokens, (all + kXK - 1) / kXK * kXK);
+    for (int64_t c = (int64_t)all * (p.dim / 8) + threadIdx.x; c < (int64_t)end * (p.dim / 8); c += kPackThreads)
+      reinterpret_cast<uint4*>(p.packed)[c] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// Joins the partial statistics of a slot along the vocabulary: `lanes` rows a block (a power of two, at
 // most 8), 256 / lanes threads a row, so that a single token's partials are read by a whole block.  The last
 // block to finish adds the blocks' sums in block order (fp64) and writes the mean or sum.
 constexpr int kJoinThreads = 256;
@@ -499,16 +692,15 @@ struct JoinParams {
   const float2* part;
   int parts;
   const float* picked;
-  const int64_t* target;
-  int64_t ignore, vocab;
-  int rows, lanes;                 // rows of this token block
+  const int* target;
+  const int* token;
+  const int* slots;
+  int slot0, rows, lanes;          // of this block of slots; rows: the most it can hold
   float* lse;
   float* row_loss;                 // losses token by token, or null
   float* out;                      // their mean or sum, or null
   int mean;
-  float* count;                    // number of counted tokens
-  double* block_loss;              // [blocks of all token blocks]
-  int* block_count;
+  double* block_loss;              // [joining blocks of all blocks of slots]
   int first_block, all_blocks;
   unsigned int* counter;
   int32_t* status;
@@ -516,15 +708,16 @@ struct JoinParams {
 __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const JoinParams p) {
   __shared__ float2 red[kJoinThreads];
   __shared__ double sum_s[kJoinThreads];
-  __shared__ int cnt_s[kJoinThreads];
   __shared__ bool last;
   pdl_launch_dependents();
   pdl_wait();
+  const int slots = *static_cast<const volatile int*>(p.slots);
+  const int rows = max(0, min(p.rows, slots - p.slot0));
   const int slices = kJoinThreads / p.lanes;
   const int r = threadIdx.x & (p.lanes - 1), slice = threadIdx.x / p.lanes;
   const int64_t row = (int64_t)blockIdx.x * p.lanes + r;
   float m = -INFINITY, s = 0.f;
-  if (row < p.rows) {
+  if (row < rows) {
 #pragma unroll 4
     for (int i = slice; i < p.parts; i += slices) {
       const float2 q = p.part[(int64_t)i * p.rows + row];
@@ -544,39 +737,23 @@ __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const JoinParam
     __syncthreads();
   }
   double sum = 0.0;
-  int cnt = 0;
-  if (slice == 0 && row < p.rows) {
+  if (slice == 0 && row < rows) {
     const float2 q = red[threadIdx.x];
     const float lse = q.x + logf(q.y);
     p.lse[row] = lse;
-    const int64_t y = p.target[row];
-    float loss = 0.f;
-    if (y != p.ignore) {
-      cnt = 1;
-      if (y >= 0 && y < p.vocab) {
-        loss = lse - p.picked[row];
-      } else {
-        loss = NAN;
-        if (p.status) atomicCAS(p.status, 0, kXBadTarget);
-      }
-    }
-    if (p.row_loss) p.row_loss[row] = loss;
+    float loss = NAN;
+    if (p.target[row] >= 0) loss = lse - p.picked[row];
+    else if (p.status) atomicCAS(p.status, 0, kXBadTarget);
+    if (p.row_loss) p.row_loss[p.token[row]] = loss;
     sum = loss;
   }
-  if (threadIdx.x < p.lanes) {
-    sum_s[threadIdx.x] = sum;
-    cnt_s[threadIdx.x] = cnt;
-  }
+  if (p.out == nullptr) return;
+  if (threadIdx.x < p.lanes) sum_s[threadIdx.x] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0.0;
-    cnt = 0;
-    for (int i = 0; i < p.lanes; ++i) {
-      sum += sum_s[i];
-      cnt += cnt_s[i];
-    }
+    for (int i = 0; i < p.lanes; ++i) sum += sum_s[i];
     p.block_loss[p.first_block + blockIdx.x] = sum;
-    p.block_count[p.first_block + blockIdx.x] = cnt;
     __threadfence();
     last = atomicAdd(p.counter, 1u) == (unsigned int)p.all_blocks - 1u;
   }
@@ -584,73 +761,80 @@ __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const JoinParam
   if (!last) return;
   __threadfence();
   sum = 0.0;
-  cnt = 0;
-  for (int i = threadIdx.x; i < p.all_blocks; i += kJoinThreads) {
-    sum += __ldcg(p.block_loss + i);
-    cnt += __ldcg(p.block_count + i);
-  }
+  for (int i = threadIdx.x; i < p.all_blocks; i += kJoinThreads) sum += __ldcg(p.block_loss + i);
   sum_s[threadIdx.x] = sum;
-  cnt_s[threadIdx.x] = cnt;
   __syncthreads();
   for (int o = kJoinThreads >> 1; o > 0; o >>= 1) {
-    if (threadIdx.x < o) {
-      sum_s[threadIdx.x] += sum_s[threadIdx.x + o];
-      cnt_s[threadIdx.x] += cnt_s[threadIdx.x + o];
-    }
+    if (threadIdx.x < o) sum_s[threadIdx.x] += sum_s[threadIdx.x + o];
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    *p.count = (float)cnt_s[0];
-    if (p.out) *p.out = (float)(p.mean ? sum_s[0] / (double)cnt_s[0] : sum_s[0]);   // no token counted: 0 / 0
-  }
+  if (threadIdx.x == 0) *p.out = (float)(p.mean ? sum_s[0] / (double)slots : sum_s[0]);   // no token counted: 0 / 0
 }
 
-// out[r, c] = sum over the slices (+ acc[r, c]), four columns a thread, slices in order.
-__global__ void __launch_bounds__(256) xent_slices_kernel(const float* __restrict__ slices, int n, int64_t slice_elems, const float* acc,
-                                                          void* out, int out_f32, int64_t total4) {
+// out[r, c] = sum over the slices (+ acc[r, c]), four columns a thread, slices in order.  `slots` (dh): the
+// rows are slots and go to their tokens' places if `token` is given.
+struct SliceParams {
+  const float* slices;
+  int n;
+  int64_t slice_elems;
+  const float* acc;
+  void* out;
+  int out_f32, rows, cols4, tokens;
+  const int* slots;
+  const int* token;
+};
+__global__ void __launch_bounds__(256) xent_slices_kernel(const SliceParams p) {
   pdl_launch_dependents();
   pdl_wait();
+  int rows = p.rows;
+  bool scatter = false;
+  if (p.slots != nullptr) {
+    rows = min(rows, *static_cast<const volatile int*>(p.slots));
+    scatter = p.token != nullptr && rows < p.tokens;
+  }
+  const int64_t total4 = (int64_t)rows * p.cols4;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total4; i += (int64_t)gridDim.x * 256) {
-    float4 v = acc ? reinterpret_cast<const float4*>(acc)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < n; ++s) {
-      const float4 f = reinterpret_cast<const float4*>(slices + s * slice_elems)[i];
+    float4 v = p.acc ? reinterpret_cast<const float4*>(p.acc)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.n; ++s) {
+      const float4 f = reinterpret_cast<const float4*>(p.slices + s * p.slice_elems)[i];
       v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
     }
-    if (out_f32) {
-      static_cast<float4*>(out)[i] = v;
+    int64_t to = i;
+    if (scatter) {
+      const int64_t r = i / p.cols4;
+      to += ((int64_t)p.token[r] - r) * p.cols4;
+    }
+    if (p.out_f32) {
+      static_cast<float4*>(p.out)[to] = v;
     } else {
       const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-      static_cast<uint2*>(out)[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      static_cast<uint2*>(p.out)[to] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
   }
 }
 
-// Column sums of dl: a block per 64 columns, 32 warps over the rows, their sums added in warp order.
-__global__ void __launch_bounds__(1024) xent_bias_grad_kernel(const __nv_bfloat16* __restrict__ dl, int64_t ld, int rows, int cols, void* db,
+// db: the column sums of dl that the gradient epilogue left per 32 slots (taken in fp32, before dl is
+// rounded).  A block per 32 columns; its 32 warps take the rows in turn and are added in warp order.
+__global__ void __launch_bounds__(1024) xent_bias_grad_kernel(const float* __restrict__ part, int64_t ld, const int* slots, int cols, void* db,
                                                               int db_f32) {
-  __shared__ float red[32][64];
+  __shared__ float red[32][32];
   pdl_launch_dependents();
   pdl_wait();
+  const int rows = (*static_cast<const volatile int*>(slots) + 31) / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 64 + 2 * lane;
-  float a = 0.f, b = 0.f;
-  if (c < cols) {                      // the pitch is even: the second element of the last pair may be padding, and is not used
+  const int c = blockIdx.x * 32 + lane;
+  float a = 0.f;
+  if (c < cols) {
 #pragma unroll 8
-    for (int r = warp; r < rows; r += 32) {
-      const uint32_t u = __ldg(reinterpret_cast<const uint32_t*>(dl + (int64_t)r * ld + c));
-      a += __uint_as_float(u << 16);
-      b += __uint_as_float(u & 0xFFFF0000u);
-    }
+    for (int r = warp; r < rows; r += 32) a += part[(int64_t)r * ld + c];
   }
-  red[warp][2 * lane] = a;
-  red[warp][2 * lane + 1] = b;
+  red[warp][lane] = a;
   __syncthreads();
-  if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < cols) {
+  if (warp == 0 && c < cols) {
     float s = 0.f;
-    for (int w = 0; w < 32; ++w) s += red[w][threadIdx.x];
-    const int at = blockIdx.x * 64 + threadIdx.x;
-    if (db_f32) static_cast<float*>(db)[at] = s;
-    else static_cast<__nv_bfloat16*>(db)[at] = __float2bfloat16_rn(s);
+    for (int w = 0; w < 32; ++w) s += red[w][lane];
+    if (db_f32) static_cast<float*>(db)[c] = s;
+    else static_cast<__nv_bfloat16*>(db)[c] = __float2bfloat16_rn(s);
   }
 }
 
@@ -722,8 +906,9 @@ int bf16_map(CUtensorMap* map, const Operand& o, int box_inner, int box_outer, C
                               (uint32_t)box_inner, (uint32_t)box_outer, sw);
 }
 
+// `packed`: the counted tokens' rows of h, read in place of operand a (kStats, kGrad) or b (kProductT)
 template <int kMode, int kBN>
-int launch_width(const Operand& a, const Operand& b, void* out, int64_t ldo, XParams g, int64_t k, cudaStream_t stream) {
+int launch_width(const Operand& a, const Operand& b, const Operand& packed, void* out, int64_t ldo, XParams g, int64_t k, cudaStream_t stream) {
   using C = XCfg<kBN>;
   constexpr bool kAMn = kMode == kProductT, kBMn = kMode == kProduct || kMode == kProductT;
   const int resident = xent_clusters<kMode, kBN>();
@@ -742,10 +927,12 @@ int launch_width(const Operand& a, const Operand& b, void* out, int64_t ldo, XPa
   }
   // the first operand's rows of a group: 32 MB, a quarter of L2
   g.group_m = (int)std::min<int64_t>(g.m_tiles, std::max<int64_t>(1, (32ll << 20) / ((int64_t)kXM * 2 * std::max<int64_t>(k, 1))));
-  CUtensorMap map_a, map_b, map_d = {};
+  CUtensorMap map_a, map_b, map_packed = {}, map_d = {};
   int rc = kAMn ? bf16_map(&map_a, a, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_a, a, kXK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == FP4T_OK)
     rc = kBMn ? bf16_map(&map_b, b, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_b, b, kXK, C::kBRows, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == FP4T_OK && kMode != kProduct)
+    rc = kBMn ? bf16_map(&map_packed, packed, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_packed, packed, kXK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == FP4T_OK && kMode != kStats) {
     const uint64_t rows = g.splits > 1 ? (uint64_t)g.splits * g.slice_rows : (uint64_t)g.rows;
     rc = encode_tensor_map_2d(&map_d, g.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, (uint64_t)g.cols, rows,
@@ -765,12 +952,13 @@ int launch_width(const Operand& a, const Operand& b, void* out, int64_t ldo, XPa
   pdl_attribute(&attr[1]);
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  FP4T_CUDA(cudaLaunchKernelEx(&cfg, xent_gemm_kernel<kMode, kBN>, map_a, map_b, map_d, g));
+  FP4T_CUDA(cudaLaunchKernelEx(&cfg, xent_gemm_kernel<kMode, kBN>, map_a, map_b, map_packed, map_d, g));
   return FP4T_OK;
 }
 template <int kMode>
-int launch_xent(int bn, const Operand& a, const Operand& b, void* out, int64_t ldo, const XParams& g, int64_t k, cudaStream_t stream) {
-  return bn == 128 ? launch_width<kMode, 128>(a, b, out, ldo, g, k, stream) : launch_width<kMode, 256>(a, b, out, ldo, g, k, stream);
+int launch_xent(int bn, const Operand& a, const Operand& b, const Operand& packed, void* out, int64_t ldo, const XParams& g, int64_t k,
+                cudaStream_t stream) {
+  return bn == 128 ? launch_width<kMode, 128>(a, b, packed, out, ldo, g, k, stream) : launch_width<kMode, 256>(a, b, packed, out, ldo, g, k, stream);
 }
 
 template <typename... Args, typename... Actual>
@@ -787,13 +975,26 @@ int launch_small(void (*kern)(Args...), int grid, int threads, cudaStream_t stre
   return FP4T_OK;
 }
 
-// One product into `out` (contiguous rows of `cols`), through slices when it is split.
+// What both passes know about the counted tokens (device memory in the workspace).
+struct Slots {
+  int* slots;
+  int* token;
+  int* target;
+  int* run_counts;
+  __nv_bfloat16* packed;
+};
+
+// One product into `out` (contiguous rows of `cols`), through slices when it is split.  to_tokens: its rows
+// are slots in the product and tokens in `out`.
 template <int kMode>
-int run_product(const Cut& cut, const Operand& a, const Operand& b, int64_t k, int64_t rows, int64_t cols, void* out, int out_f32,
-                const float* acc, float* slices, int32_t* status, cudaStream_t stream) {
+int run_product(const Cut& cut, const Operand& a, const Operand& b, const Operand& packed, int64_t k, int64_t rows, int64_t cols, int64_t tokens,
+                void* out, int out_f32, bool to_tokens, const float* acc, float* slices, const Slots& sl, int32_t* status, cudaStream_t stream) {
   XParams g = {};
   g.rows = (int)rows;
   g.cols = (int)cols;
+  g.tokens = (int)tokens;
+  g.slots = sl.slots;
+  g.token = sl.token;
   g.status = status;
   g.out_f32 = out_f32;
   g.splits = cut.splits;
@@ -801,50 +1002,112 @@ int run_product(const Cut& cut, const Operand& a, const Operand& b, int64_t k, i
   if (cut.splits == 1) {
     g.acc = acc;
     g.ldacc = cols;
-    return launch_xent<kMode>(cut.bn, a, b, out, cols, g, k, stream);
+    g.out = to_tokens ? out : nullptr;
+    return launch_xent<kMode>(cut.bn, a, b, packed, out, cols, g, k, stream);
   }
   g.slice_rows = (int)cut.slice_rows;
   g.out_f32 = 1;
-  int rc = launch_xent<kMode>(cut.bn, a, b, slices, cols, g, k, stream);
+  int rc = launch_xent<kMode>(cut.bn, a, b, packed, slices, cols, g, k, stream);
   if (rc != FP4T_OK) return rc;
-  const int64_t total4 = rows * cols / 4;
-  const int grid = (int)std::min<int64_t>(ceil_div(total4, 256), 148 * 8);
-  return launch_small(xent_slices_kernel, grid, 256, stream, (const float*)slices, cut.splits, cut.slice_rows * cols, acc, out, out_f32, total4);
+  SliceParams p = {};
+  p.slices = slices;
+  p.n = cut.splits;
+  p.slice_elems = cut.slice_rows * cols;
+  p.acc = acc;
+  p.out = out;
+  p.out_f32 = out_f32;
+  p.rows = (int)rows;
+  p.cols4 = (int)(cols / 4);
+  p.tokens = (int)tokens;
+  p.slots = kMode == kProduct ? sl.slots : nullptr;
+  p.token = to_tokens ? sl.token : nullptr;
+  const int grid = (int)std::min<int64_t>(ceil_div(rows * cols / 4, 256), 148 * 8);
+  return launch_small(xent_slices_kernel, grid, 256, stream, p);
 }
 
 int64_t round_up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
 
 int width_for(int64_t vocab) { return vocab <= 128 ? 128 : 256; }   // of a tile of logits
 
-// Forward workspace: counter, block sums and counts, the targets' logits, partial statistics.
-struct ForwardPlan {
-  int64_t block, parts, join_blocks;      // tokens per block, partials per token, joining blocks of all token blocks
-  int lanes;
-  int64_t o_loss, o_count, o_picked, o_part, bytes;
+// Slots in the workspace: their number, the token and target of each, counts per run, the packed rows of h.
+struct SlotPlan {
+  int64_t run, runs, o_token, o_target, o_runs, o_packed, bytes;
 };
-ForwardPlan plan_forward(int64_t tokens, int64_t vocab) {
+SlotPlan plan_slots(int64_t tokens, int64_t dim) {
+  SlotPlan p;
+  p.run = std::max<int64_t>(32, round_up(ceil_div(tokens, 148 * 4), 32));
+  p.runs = ceil_div(tokens, p.run);
+  p.o_token = 256;                       // slot count at 0, joining kernel's counter at 128
+  p.o_target = p.o_token + round_up(tokens * 4, 128);
+  p.o_runs = p.o_target + round_up(tokens * 4, 128);
+  p.o_packed = round_up(p.o_runs + p.runs * 4, 1024);
+  p.bytes = p.o_packed + round_up(tokens * dim * 2, 1024);
+  return p;
+}
+Slots slots_at(uint8_t* ws, const SlotPlan& p) {
+  return Slots{reinterpret_cast<int*>(ws), reinterpret_cast<int*>(ws + p.o_token), reinterpret_cast<int*>(ws + p.o_target),
+               reinterpret_cast<int*>(ws + p.o_runs), reinterpret_cast<__nv_bfloat16*>(ws + p.o_packed)};
+}
+int launch_pack(const SlotPlan& plan, const Slots& sl, const void* h, int64_t ldh, const int64_t* target, int64_t tokens, int64_t dim, int64_t vocab,
+                int64_t ignore, float* row_loss, void* dh, int dh_f32, unsigned int* counter, float* count, cudaStream_t stream) {
+  PackParams p = {};
+  p.target = target;
+  p.ignore = ignore;
+  p.vocab = (int)vocab;
+  p.tokens = (int)tokens;
+  p.run = (int)plan.run;
+  p.h = static_cast<const __nv_bfloat16*>(h);
+  p.ldh = ldh;
+  p.dim = (int)dim;
+  p.packed = sl.packed;
+  p.slots = sl.slots;
+  p.token = sl.token;
+  p.slot_target = sl.target;
+  p.row_loss = row_loss;
+  p.dh = dh;
+  p.dh_f32 = dh_f32;
+  p.counter = counter;
+  p.count = count;
+  if (tokens > kPackSelf) {
+    p.run_counts = sl.run_counts;
+    const int rc = launch_small(xent_run_count_kernel, (int)plan.runs, kPackThreads, stream, target, ignore, (int)tokens, (int)plan.run, sl.run_counts);
+    if (rc != FP4T_OK) return rc;
+  }
+  return launch_small(xent_pack_kernel, (int)plan.runs, kPackThreads, stream, p);
+}
+
+// Forward workspace: slots, the joining blocks' sums, the targets' logits, partial statistics of a block of slots.
+struct ForwardPlan {
+  SlotPlan slots;
+  int64_t block, parts, join_blocks;      // slots per block, partials per slot, joining blocks of all blocks of slots
+  int lanes;
+  int64_t o_loss, o_picked, o_part, bytes;
+};
+ForwardPlan plan_forward(int64_t tokens, int64_t dim, int64_t vocab) {
   ForwardPlan p;
+  p.slots = plan_slots(tokens, dim);
   p.block = std::min(tokens, kTokenBlock);
   p.parts = 2 * ceil_div(vocab, width_for(vocab));
   p.lanes = 1;
   while (p.lanes < 8 && p.lanes < tokens) p.lanes <<= 1;
   p.join_blocks = (tokens / p.block) * ceil_div(p.block, p.lanes) + ceil_div(tokens % p.block, p.lanes);
-  p.o_loss = 128;
-  p.o_count = p.o_loss + round_up(p.join_blocks * 8, 128);
-  p.o_picked = p.o_count + round_up(p.join_blocks * 4, 128);
+  p.o_loss = p.slots.bytes;
+  p.o_picked = p.o_loss + round_up(p.join_blocks * 8, 128);
   p.o_part = p.o_picked + round_up(p.block * 4, 128);
   p.bytes = p.o_part + p.parts * p.block * 8;
   return p;
 }
 
-// Backward workspace: dl of a piece, dh in fp32 when there are several pieces, K slices.
+// Backward workspace: slots, dl of a piece, dh in fp32 when there are several pieces, column sums, K slices.
 struct BackwardPlan {
+  SlotPlan slots;
   int64_t piece, pieces, ld;
   Cut dh, dw;
-  int64_t o_acc, o_slices, bytes;
+  int64_t o_dl, o_acc, o_cols, o_slices, bytes;
 };
-BackwardPlan plan_backward(int64_t tokens, int64_t dim, int64_t vocab, bool want_dh, bool want_dw, int clusters) {
+BackwardPlan plan_backward(int64_t tokens, int64_t dim, int64_t vocab, bool want_dh, bool want_dw, bool want_db, int clusters) {
   BackwardPlan p;
+  p.slots = plan_slots(tokens, dim);
   p.piece = std::min(round_up(vocab, 256), std::max(kMinPiece, kPieceBytes / (2 * tokens) / 256 * 256));
   p.pieces = ceil_div(vocab, p.piece);
   p.piece = round_up(ceil_div(vocab, p.pieces), 256);       // even pieces
@@ -852,8 +1115,10 @@ BackwardPlan plan_backward(int64_t tokens, int64_t dim, int64_t vocab, bool want
   p.ld = std::min(p.piece, round_up(vocab, 8));
   p.dh = cut_product(tokens, dim, std::min(p.piece, vocab), true, clusters);
   p.dw = cut_product(std::min(p.piece, vocab), dim, tokens, true, clusters);
-  p.o_acc = round_up(tokens * p.ld * 2, 1024);
-  p.o_slices = p.o_acc + (want_dh && p.pieces > 1 ? round_up(tokens * dim * 4, 1024) : 0);
+  p.o_dl = p.slots.bytes;
+  p.o_acc = p.o_dl + round_up(tokens * p.ld * 2, 1024);
+  p.o_cols = p.o_acc + (want_dh && p.pieces > 1 ? round_up(tokens * dim * 4, 1024) : 0);
+  p.o_slices = p.o_cols + (want_db ? round_up(round_up(tokens, kXK) / 32 * p.ld * 4, 1024) : 0);
   p.bytes = p.o_slices + std::max(want_dh ? p.dh.slice_bytes(dim) : 0, want_dw ? p.dw.slice_bytes(dim) : 0);
   return p;
 }
@@ -886,9 +1151,9 @@ FP4T_DEFINE_WAIT_TIMEOUT_SETTER(set_wait_timeout_xent)
 
 using namespace fp4t;
 
-extern "C" int64_t fp4t_linear_xent_forward_workspace_bytes(int64_t tokens, int64_t vocab) {
-  if (check_sizes("fp4t_linear_xent_forward_workspace_bytes", tokens, 8, vocab) != FP4T_OK) return -1;
-  return tokens == 0 ? 128 : plan_forward(tokens, vocab).bytes;
+extern "C" int64_t fp4t_linear_xent_forward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocab) {
+  if (check_sizes("fp4t_linear_xent_forward_workspace_bytes", tokens, dim, vocab) != FP4T_OK) return -1;
+  return tokens == 0 ? 128 : plan_forward(tokens, dim, vocab).bytes;
 }
 
 extern "C" int fp4t_linear_xent_forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const void* bias, int bias_dtype,
@@ -902,47 +1167,52 @@ extern "C" int fp4t_linear_xent_forward(const void* h, int64_t ldh, const void* 
   rc = check_inputs(name, h, ldh, w, ldw, bias, bias_dtype, target, dim, reduction, workspace);
   if (rc != FP4T_OK) return rc;
   FP4T_REQUIRE(loss && lse && count, "%s: null pointer", name);
-  const ForwardPlan p = plan_forward(tokens, vocab);
+  const ForwardPlan p = plan_forward(tokens, dim, vocab);
   FP4T_REQUIRE(workspace_bytes >= p.bytes, "%s: the workspace holds %lld bytes of %lld", name, (long long)workspace_bytes, (long long)p.bytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (!status) status = current_status_word();
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const Slots sl = slots_at(ws, p.slots);
+  unsigned int* counter = reinterpret_cast<unsigned int*>(ws + 128);
+  rc = launch_pack(p.slots, sl, h, ldh, target, tokens, dim, vocab, ignore_index, reduction == FP4T_XENT_NONE ? loss : nullptr, nullptr, 0, counter,
+                   count, s);
+  if (rc != FP4T_OK) return rc;
   int64_t first_block = 0;
   for (int64_t t0 = 0; t0 < tokens; t0 += p.block) {
     const int64_t rows = std::min(p.block, tokens - t0);
     XParams g = {};
     g.rows = (int)rows;
     g.cols = (int)vocab;
+    g.tokens = (int)tokens;
+    g.slots = sl.slots;
+    g.slot0 = (int)t0;
     g.bias = bias;
     g.bias_f32 = bias_dtype == FP4T_DT_F32;
-    g.target = target + t0;
-    g.ignore = ignore_index;
+    g.target = sl.target + t0;
     g.part = reinterpret_cast<float2*>(ws + p.o_part);
     g.picked = reinterpret_cast<float*>(ws + p.o_picked);
-    g.counter = reinterpret_cast<unsigned int*>(ws + (t0 == 0 ? 0 : 64));      // counts over all token blocks: zeroed by the first
     g.status = status;
     rc = launch_xent<kStats>(width_for(vocab), Operand{static_cast<const __nv_bfloat16*>(h) + t0 * ldh, rows, dim, ldh}, Operand{w, vocab, dim, ldw},
-                             nullptr, 0, g, dim, s);
+                             Operand{sl.packed + t0 * dim, rows, dim, dim}, nullptr, 0, g, dim, s);
     if (rc != FP4T_OK) return rc;
     JoinParams j = {};
     j.part = g.part;
     j.parts = (int)p.parts;
     j.picked = g.picked;
     j.target = g.target;
-    j.ignore = ignore_index;
-    j.vocab = vocab;
+    j.token = sl.token + t0;
+    j.slots = sl.slots;
+    j.slot0 = (int)t0;
     j.rows = (int)rows;
     j.lanes = p.lanes;
     j.lse = lse + t0;
-    j.row_loss = reduction == FP4T_XENT_NONE ? loss + t0 : nullptr;
+    j.row_loss = reduction == FP4T_XENT_NONE ? loss : nullptr;
     j.out = reduction == FP4T_XENT_NONE ? nullptr : loss;
     j.mean = reduction == FP4T_XENT_MEAN;
-    j.count = count;
     j.block_loss = reinterpret_cast<double*>(ws + p.o_loss);
-    j.block_count = reinterpret_cast<int*>(ws + p.o_count);
     j.first_block = (int)first_block;
     j.all_blocks = (int)p.join_blocks;
-    j.counter = reinterpret_cast<unsigned int*>(ws);
+    j.counter = counter;
     j.status = status;
     const int blocks = (int)ceil_div(rows, p.lanes);
     first_block += blocks;
@@ -952,25 +1222,25 @@ extern "C" int fp4t_linear_xent_forward(const void* h, int64_t ldh, const void* 
   return FP4T_OK;
 }
 
-extern "C" int64_t fp4t_linear_xent_backward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocab, int want_dh, int want_dw) {
+extern "C" int64_t fp4t_linear_xent_backward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocab, int want_dh, int want_dw,
+                                                              int want_db) {
   if (check_sizes("fp4t_linear_xent_backward_workspace_bytes", tokens, dim, vocab) != FP4T_OK) return -1;
   const int clusters = cluster_budget();
   if (tokens == 0 || clusters <= 0) return tokens == 0 ? 128 : -1;
-  return plan_backward(tokens, dim, vocab, want_dh != 0, want_dw != 0, clusters).bytes;
+  return plan_backward(tokens, dim, vocab, want_dh != 0, want_dw != 0, want_db != 0, clusters).bytes;
 }
 
 extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, int64_t ldh, const void* w, int64_t ldw, const void* bias,
-                                         int bias_dtype, const int64_t* target, const float* lse, const float* count, int64_t tokens,
-                                         int64_t dim, int64_t vocab, int64_t ignore_index, int reduction, void* dh, int dh_dtype, void* dw,
-                                         int dw_dtype, void* db, int db_dtype, void* workspace, int64_t workspace_bytes, int32_t* status,
-                                         fp4t_stream_t stream) {
+                                         int bias_dtype, const int64_t* target, const float* lse, int64_t tokens, int64_t dim, int64_t vocab,
+                                         int64_t ignore_index, int reduction, void* dh, int dh_dtype, void* dw, int dw_dtype, void* db,
+                                         int db_dtype, void* workspace, int64_t workspace_bytes, int32_t* status, fp4t_stream_t stream) {
   const char* name = "fp4t_linear_xent_backward";
   int rc = check_sizes(name, tokens, dim, vocab);
   if (rc != FP4T_OK) return rc;
   FP4T_REQUIRE(tokens > 0, "%s: no tokens", name);
   rc = check_inputs(name, h, ldh, w, ldw, bias, bias_dtype, target, dim, reduction, workspace);
   if (rc != FP4T_OK) return rc;
-  FP4T_REQUIRE(grad_loss && lse && count, "%s: null pointer", name);
+  FP4T_REQUIRE(grad_loss && lse, "%s: null pointer", name);
   FP4T_REQUIRE((!dh || dh_dtype == FP4T_DT_F32 || dh_dtype == FP4T_DT_BF16) && (!dw || dw_dtype == FP4T_DT_F32 || dw_dtype == FP4T_DT_BF16) &&
                    (!db || db_dtype == FP4T_DT_F32 || db_dtype == FP4T_DT_BF16),
                "%s: gradients must be f32 or bf16", name);
@@ -981,31 +1251,39 @@ extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, 
     set_error("%s: the current device is not an sm_100 part", name);
     return FP4T_ERR_DEVICE;
   }
-  const BackwardPlan p = plan_backward(tokens, dim, vocab, dh != nullptr, dw != nullptr, clusters);
+  const BackwardPlan p = plan_backward(tokens, dim, vocab, dh != nullptr, dw != nullptr, db != nullptr, clusters);
   FP4T_REQUIRE(workspace_bytes >= p.bytes, "%s: the workspace holds %lld bytes of %lld", name, (long long)workspace_bytes, (long long)p.bytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (!status) status = current_status_word();
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  __nv_bfloat16* dl = reinterpret_cast<__nv_bfloat16*>(ws);
+  const Slots sl = slots_at(ws, p.slots);
+  rc = launch_pack(p.slots, sl, h, ldh, target, tokens, dim, vocab, ignore_index, nullptr, dh, dh_dtype == FP4T_DT_F32, nullptr, nullptr, s);
+  if (rc != FP4T_OK) return rc;
+  __nv_bfloat16* dl = reinterpret_cast<__nv_bfloat16*>(ws + p.o_dl);
   float* acc = reinterpret_cast<float*>(ws + p.o_acc);
   float* slices = reinterpret_cast<float*>(ws + p.o_slices);
+  const Operand hop{h, tokens, dim, ldh}, packed{sl.packed, tokens, dim, dim};
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, vc = std::min(p.piece, vocab - v0);
-    const Operand hop{h, tokens, dim, ldh}, wop{static_cast<const __nv_bfloat16*>(w) + v0 * ldw, vc, dim, ldw}, dop{dl, tokens, vc, p.ld};
+    const Operand wop{static_cast<const __nv_bfloat16*>(w) + v0 * ldw, vc, dim, ldw}, dop{dl, tokens, vc, p.ld};
     XParams g = {};
     g.rows = (int)tokens;
     g.cols = (int)vc;
+    g.tokens = (int)tokens;
+    g.slots = sl.slots;
+    g.token = sl.token;
     g.bias = bias ? static_cast<const uint8_t*>(bias) + v0 * (bias_dtype == FP4T_DT_F32 ? 4 : 2) : nullptr;
     g.bias_f32 = bias_dtype == FP4T_DT_F32;
-    g.target = target;
-    g.ignore = ignore_index;
-    g.col0 = v0;
+    g.target = sl.target;
+    g.col0 = (int)v0;
     g.lse = lse;
     g.grad = grad_loss;
     g.grad_per_row = reduction == FP4T_XENT_NONE;
-    g.count = reduction == FP4T_XENT_MEAN ? count : nullptr;
+    g.mean = reduction == FP4T_XENT_MEAN;
+    g.col_part = db ? reinterpret_cast<float*>(ws + p.o_cols) : nullptr;
+    g.col_ld = p.ld;
     g.status = status;
-    rc = launch_xent<kGrad>(width_for(vc), hop, wop, dl, p.ld, g, dim, s);
+    rc = launch_xent<kGrad>(width_for(vc), hop, wop, packed, dl, p.ld, g, dim, s);
     if (rc != FP4T_OK) return rc;
     if (dh) {
       const bool last = i == p.pieces - 1;
@@ -1015,18 +1293,18 @@ extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, 
         cut.ks_per_split = (int)std::min<int64_t>(cut.ks_per_split, stages);
         cut.splits = (int)std::min<int64_t>(cut.splits, ceil_div(stages, cut.ks_per_split));
       }
-      rc = run_product<kProduct>(cut, dop, wop, vc, tokens, dim, last ? dh : static_cast<void*>(acc), last ? dh_dtype == FP4T_DT_F32 : 1,
-                                 i > 0 ? acc : nullptr, slices, status, s);
+      rc = run_product<kProduct>(cut, dop, wop, packed, vc, tokens, dim, tokens, last ? dh : static_cast<void*>(acc),
+                                 last ? dh_dtype == FP4T_DT_F32 : 1, last, i > 0 ? acc : nullptr, slices, sl, status, s);
       if (rc != FP4T_OK) return rc;
     }
     if (dw) {
       void* out = static_cast<uint8_t*>(dw) + v0 * dim * (dw_dtype == FP4T_DT_F32 ? 4 : 2);
-      rc = run_product<kProductT>(p.dw, dop, hop, tokens, vc, dim, out, dw_dtype == FP4T_DT_F32, nullptr, slices, status, s);
+      rc = run_product<kProductT>(p.dw, dop, hop, packed, tokens, vc, dim, tokens, out, dw_dtype == FP4T_DT_F32, false, nullptr, slices, sl, status, s);
       if (rc != FP4T_OK) return rc;
     }
     if (db) {
       void* out = static_cast<uint8_t*>(db) + v0 * (db_dtype == FP4T_DT_F32 ? 4 : 2);
-      rc = launch_small(xent_bias_grad_kernel, (int)ceil_div(vc, 64), 1024, s, (const __nv_bfloat16*)dl, p.ld, (int)tokens, (int)vc, out,
+      rc = launch_small(xent_bias_grad_kernel, (int)ceil_div(vc, 32), 1024, s, (const float*)g.col_part, p.ld, (const int*)sl.slots, (int)vc, out,
                         (int)(db_dtype == FP4T_DT_F32));
       if (rc != FP4T_OK) return rc;
     }

@@ -35,16 +35,16 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         h = _operand(hidden.reshape(-1, hidden.shape[-1]), "hidden")
         w = _operand(weight, "weight")
         t = target.reshape(-1)
-        loss, lse, count = _ops.linear_cross_entropy_forward(h, w, bias, t, ignore_index, reduction)
-        ctx.save_for_backward(h, w, bias, t, lse, count)
+        loss, lse, _ = _ops.linear_cross_entropy_forward(h, w, bias, t, ignore_index, reduction)
+        ctx.save_for_backward(h, w, bias, t, lse)
         return loss.view(target.shape) if reduction == "none" else loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        h, w, bias, t, lse, count = ctx.saved_tensors
+        h, w, bias, t, lse = ctx.saved_tensors
         want = [dt if need else None for dt, need in zip(ctx.dtypes, ctx.needs_input_grad)]
-        dh, dw, db = _ops.linear_cross_entropy_backward(grad.reshape(-1), h, w, bias, t, lse, count, *ctx.args, *want)
+        dh, dw, db = _ops.linear_cross_entropy_backward(grad.reshape(-1), h, w, bias, t, lse, *ctx.args, *want)
         return None if dh is None else dh.view(ctx.shape), dw, db, None, None, None
 
 

@@ -532,32 +532,33 @@ FP4T_API int fp4t_qk_norm_rotary_backward(const fp4t_heads_t* dy, const fp4t_hea
  * bias [vocab] f32 or bf16, or null; target [tokens] int64.  Tokens whose target is ignore_index have loss
  * 0, count for nothing in the mean and get zero gradients.  A target outside [0, vocab) that is not
  * ignore_index makes its token's loss NaN and leaves 41 in the status word.  With FP4T_XENT_MEAN and no
- * counted token the loss is NaN (0 / 0) and the gradients are zero.  Pointers are 16-byte aligned,
+ * counted token the loss is NaN (0 / 0) and the gradients are zero.  Ignored tokens cost no products (the
+ * counted ones are packed together on the device) and nothing of their rows of h reaches a result.  Pointers are 16-byte aligned,
  * tokens >= 1.  Losses, lse and sums in fp32 (the mean's sum in fp64); logits are accumulated in fp32.
  *
- * forward:  loss [1], or [tokens] with FP4T_XENT_NONE; lse [tokens] and count [1] (fp32) for the backward pass.
+ * forward:  loss [1], or [tokens] with FP4T_XENT_NONE; lse [tokens] for the backward
+ *   pass (of the counted tokens, in order); count [1]: how many were counted (fp32).
  * backward: any of dh [tokens, dim], dw [vocab, dim] and db [vocab] (contiguous, f32 or bf16; null: not
  *   wanted) from grad_loss ([1], or [tokens] with FP4T_XENT_NONE).  The logits' gradient is rounded to bf16,
- *   the operand type of the products, and to nothing else; they accumulate in fp32.
+ *   the operand type of the two products, which accumulate in fp32; db sums it before that rounding.
  * Workspaces: 16-byte aligned, sizes from the two calls below (the backward one holds dl of one
  * piece, at most 512 MB or 4096 entries wide).  All results are reproducible.
  */
 enum { FP4T_XENT_NONE = 0, FP4T_XENT_MEAN = 1, FP4T_XENT_SUM = 2 };
-FP4T_API int64_t fp4t_linear_xent_forward_workspace_bytes(int64_t tokens, int64_t vocab);
+FP4T_API int64_t fp4t_linear_xent_forward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocab);
 FP4T_API int fp4t_linear_xent_forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const void* bias,
                                       int bias_dtype, const int64_t* target, int64_t tokens, int64_t dim,
                                       int64_t vocab, int64_t ignore_index, int reduction, float* loss,
                                       float* lse, float* count, void* workspace, int64_t workspace_bytes,
                                       int32_t* status, fp4t_stream_t stream);
 FP4T_API int64_t fp4t_linear_xent_backward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocab, int want_dh,
-                                                           int want_dw);
+                                                           int want_dw, int want_db);
 FP4T_API int fp4t_linear_xent_backward(const float* grad_loss, const void* h, int64_t ldh, const void* w,
                                        int64_t ldw, const void* bias, int bias_dtype, const int64_t* target,
-                                       const float* lse, const float* count, int64_t tokens, int64_t dim,
-                                       int64_t vocab, int64_t ignore_index, int reduction, void* dh,
-                                       int dh_dtype, void* dw, int dw_dtype, void* db, int db_dtype,
-                                       void* workspace, int64_t workspace_bytes, int32_t* status,
-                                       fp4t_stream_t stream);
+                                       const float* lse, int64_t tokens, int64_t dim, int64_t vocab,
+                                       int64_t ignore_index, int reduction, void* dh, int dh_dtype, void* dw,
+                                       int dw_dtype, void* db, int db_dtype, void* workspace,
+                                       int64_t workspace_bytes, int32_t* status, fp4t_stream_t stream);
 
 /* Byte-matrix transpose [rows, cols] -> [cols, rows] (E4M3 codes for the NN / NT operand
  * forms of custom/backend/csrc/cublaslt_mm_mxfp8.cu:70-88). */

@@ -31,6 +31,9 @@ CASES = [
     (1111, 1032, 777, None, "sum", 0.9),
     (40000, 64, 9000, BF16, "mean", 0.1),      # several blocks of tokens, several pieces of the vocabulary
     (20000, 8, 27000, None, "mean", 0.0),      # pieces and splits together
+    (20000, 16, 27000, F32, "none", 0.7),      # the same with most tokens ignored: whole blocks of slots are empty
+    (33000, 64, 500, None, "mean", 0.995),     # a few slots left of many tokens; per-run counts
+    (3, 64, 500, None, "sum", 0.7),
 ]
 
 
@@ -60,6 +63,7 @@ def reference(h, w, b, t, reduction, grad):
     p = x.sub_(lse[:, None]).exp_()
     ex = D * 2.0 ** -23 * float((H.abs() @ W.abs().T).max())
     e = p * gr.abs() * (2 * ex + 2.0 ** -17)
+    eb = e.sum(0)                                # db is summed before the rounding
     dl = p.mul_(gr).scatter_add_(1, y, -gr)
     e += dl.abs() * 2.0 ** -8
     res = {"loss": out, "loss_tol": (2 * ex + 2.0 ** -18) * (1 if reduction != "sum" else max(1, int(n))) + 2.0 ** -18 * out.abs()}
@@ -67,7 +71,7 @@ def reference(h, w, b, t, reduction, grad):
     a = dl.abs_()
     res["dh_tol"] = e @ W.abs() + V * 2.0 ** -23 * (a @ W.abs())
     res["dw_tol"] = e.T @ H.abs() + T * 2.0 ** -23 * (a.T @ H.abs())
-    res["db_tol"] = e.sum(0) + T * 2.0 ** -23 * a.sum(0)
+    res["db_tol"] = eb + T * 2.0 ** -23 * a.sum(0)
     return res
 
 
@@ -103,7 +107,8 @@ def test_loss_and_gradients(case):
     hd, wd = h.detach(), w.detach()
     bd = None if b is None else b.detach()
     _, lse, count = ops.linear_cross_entropy_forward(hd, wd, bd, t, -100, reduction)
-    only = ops.linear_cross_entropy_backward(grad, hd, wd, bd, t, lse, count, -100, reduction, dw_dtype=BF16)
+    assert float(count) == int((t != -100).sum())
+    only = ops.linear_cross_entropy_backward(grad, hd, wd, bd, t, lse, -100, reduction, dw_dtype=BF16)
     assert only[0] is None and only[2] is None and torch.equal(only[1], grads[1])
     ops.check_status()
 
@@ -200,6 +205,18 @@ def test_masked_entries_infinities_and_nan():
     t2[3:5] = -100
     out = linear_cross_entropy(bad, w, t2, b, reduction="none")
     assert (out[3:5] == 0).all() and torch.equal(out[5:], got[5:])
+    # the ignored tokens' garbage reaches no gradient: as if they were not there
+    for dt in (BF16, F32):
+        bl2 = b.clone().requires_grad_()
+        with torch.autocast("cuda", dtype=BF16):
+            got1 = torch.autograd.grad(linear_cross_entropy(bad.to(dt).requires_grad_(), wl, t2, bl2), [wl, bl2])
+            leaf = bad.to(dt).requires_grad_()
+            (got2,) = torch.autograd.grad(linear_cross_entropy(leaf, wl, t2, b), leaf)
+            keep = torch.cat([torch.arange(3), torch.arange(5, T)]).cuda()
+            rest = h[keep].to(dt).requires_grad_()
+            want1 = torch.autograd.grad(linear_cross_entropy(rest, wl, t[keep], bl2), [rest, wl, bl2])
+        assert torch.equal(got1[0], want1[1]) and torch.equal(got1[1], want1[2])
+        assert (got2[3:5] == 0).all() and torch.equal(got2[keep], want1[0])
     out = linear_cross_entropy(bad, w, t, b, reduction="none")
     assert out[3].isnan() and out[4].isnan() and torch.equal(out[5:], got[5:])
 

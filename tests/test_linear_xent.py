@@ -27,7 +27,7 @@ def test_argument_errors_of_the_c_entries():
         return L.fp4t_linear_xent_forward(h, ldh, w, ldw, bias, bd, target, T, D, V, -100, red, loss, buf, buf, ws, n, None, None)
 
     def bwd(h=buf, ldh=64, T=4, D=64, V=10, red=1, dh=buf, dt=0, grad=buf, n=1 << 40):
-        return L.fp4t_linear_xent_backward(grad, h, ldh, buf, 64, None, 0, buf, buf, buf, T, D, V, -100, red, dh, dt, None, 0, None, 0,
+        return L.fp4t_linear_xent_backward(grad, h, ldh, buf, 64, None, 0, buf, buf, T, D, V, -100, red, dh, dt, None, 0, None, 0,
                                            buf, n, None, None)
 
     for kw, word in ((dict(T=-1), "shape"), (dict(T=0), "tokens"), (dict(V=0), "shape"), (dict(D=60, ldh=64), "multiple of 8"), (dict(D=0), "shape"),
@@ -43,7 +43,7 @@ def test_argument_errors_of_the_c_entries():
         assert word in L.fp4t_last_error().decode(), kw
     assert bwd(dh=None) == 0                                    # nothing wanted, nothing launched
     size = L.fp4t_linear_xent_forward_workspace_bytes
-    assert size(0, 10) == 128 and size(-1, 10) == -1 and size(10, 0) == -1
-    # at most 16384 tokens' partial statistics at once: two numbers per 128 entries
-    assert size(10 ** 6, 131072) < 1024 * 16384 * 8 + (1 << 22)
-    assert size(1, 131072) < 1 << 15
+    assert size(0, 8, 10) == 128 and size(-1, 8, 10) == -1 and size(10, 8, 0) == -1 and size(10, 9, 10) == -1
+    # at most 16384 tokens' partial statistics at once (two numbers per 128 entries), and the packed rows
+    assert size(10 ** 6, 64, 131072) < 1024 * 16384 * 8 + 10 ** 6 * (128 + 16) + (1 << 22)
+    assert size(1, 64, 131072) < 1 << 15

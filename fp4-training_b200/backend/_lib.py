@@ -24,11 +24,6 @@ _c_i64 = ctypes.c_int64
 _c_vp = ctypes.c_void_p
 
 
-class Heads(ctypes.Structure):
-    """fp4t_heads_t: one [batch, tokens, heads, head_dim] tensor, strides in elements."""
-    _fields_ = [("data", _c_vp), ("heads", _c_i64), ("stride_batch", _c_i64), ("stride_token", _c_i64), ("stride_head", _c_i64)]
-
-
 class Rotary(ctypes.Structure):
     """fp4t_rotary_t: positions and the table of turning pairs."""
     _fields_ = [("positions", _c_vp), ("positions_i64", ctypes.c_int), ("stride_batch", _c_i64), ("stride_token", _c_i64),
@@ -36,8 +31,9 @@ class Rotary(ctypes.Structure):
                 ("turns", _c_vp), ("axis", _c_vp)]
 
 
-_p_heads = ctypes.POINTER(Heads)
-_p_rotary = ctypes.POINTER(Rotary)
+# addresses of one to six fp4t_heads_t in a row (int64 fields: data, heads, stride_batch, stride_token,
+# stride_head), of a Rotary
+_p_heads = _p_rotary = _c_vp
 _p_vps = ctypes.POINTER(_c_vp)
 
 _SIGNATURES = {

@@ -530,99 +530,136 @@ def layernorm_backward(dy, x, mean, rstd, gamma):
 
 
 # ------------------------------------------------------------------ rotary positions, query / key norms
-def _heads_args(what, tensors, like=None):
-    """Checks 4-D [batch, tokens, heads, head_dim] tensors of one dtype and device; unit column stride."""
-    out = []
-    first = like if like is not None else tensors[0]
-    for i, t in enumerate(tensors):
+# These calls take a few microseconds of GPU time on a decoding step's tensors, so the host's share is kept
+# small: sizes and strides go over in one array, and nothing is looked up twice.
+_I64 = ctypes.c_int64
+_HEADS = {n: _I64 * (5 * n) for n in range(1, 7)}        # n fp4t_heads_t in a row
+
+
+class _Current(contextlib.AbstractContextManager):
+    """The context of a device that is already current."""
+
+    def __exit__(self, *exc):
+        return None
+
+
+_CURRENT = _Current()
+
+
+def _device_context(index):
+    return _CURRENT if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def _heads(what, tensors, like=None):
+    """Checks one or two [batch, tokens, heads, head_dim] tensors of one dtype, device and shape but for the
+    heads; -> (tensors with unit column stride, the fields of their fp4t_heads_t)."""
+    first = tensors[0] if like is None else like
+    dt, dev, shape = first.dtype, first.device, first.shape
+    if dt is not torch.bfloat16 and dt is not torch.float32:
+        _need_cuda(first)
+        raise ValueError(f"{what} runs on float32 / bfloat16 tensors")
+    out, fields = [], []
+    for t in tensors:
+        if not t.is_cuda:
+            _need_cuda(t)
         if t.ndim != 4:
             raise ValueError(f"{what} takes [batch, tokens, heads, head_dim] tensors")
-        if t.dtype != first.dtype or t.device != first.device:
-            raise ValueError(f"{what}: all tensors must have one dtype and one device")
-        if t.shape[:2] != first.shape[:2] or t.shape[3] != first.shape[3]:
-            raise ValueError(f"{what}: tensors must agree in batch, tokens and head_dim")
-        out.append(t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous())
+        if t is not first:
+            if t.dtype is not dt or t.device != dev:
+                raise ValueError(f"{what}: all tensors must have one dtype and one device")
+            sh = t.shape
+            if sh[0] != shape[0] or sh[1] != shape[1] or sh[3] != shape[3]:
+                raise ValueError(f"{what}: tensors must agree in batch, tokens and head_dim")
+        sb, st, hs, unit = t.stride()
+        if unit != 1:
+            t = t.contiguous()
+            sb, st, hs, _ = t.stride()
+        out.append(t)
+        fields += (t.data_ptr(), t.shape[2], sb, st, hs)
+    return out, fields
+
+
+def _outputs(x, fields):
+    """Contiguous results of x's shapes; their fp4t_heads_t fields are appended."""
+    out = []
+    for t in x:
+        y = t.new_empty(t.shape)
+        _, L, H, D = t.shape
+        fields += (y.data_ptr(), H, L * H * D, H * D, D)
+        out.append(y)
     return out
-
-
-def _heads_array(tensors):
-    arr = (_lib.Heads * len(tensors))()
-    for a, t in zip(arr, tensors):
-        a.data, a.heads = t.data_ptr(), t.shape[2]
-        a.stride_batch, a.stride_token, a.stride_head, _ = t.stride()
-    return arr
 
 
 def _rotary_args(what, x, positions, table):
     """fp4t_rotary_t of a call.  table: (turns int64 [pairs], axis int32 [pairs], axes, interleaved) or None."""
-    r = _lib.Rotary()
     if table is None:
         if positions is not None:
             raise ValueError(f"{what}: positions without a rotary table")
-        return r
+        return _lib.Rotary()
     turns, axis, axes, interleaved = table
     if positions is None:
         raise ValueError(f"{what}: a rotary table needs positions")
-    _need_cuda(positions, turns, axis)
-    if positions.dtype not in (torch.int32, torch.int64):
+    if not (positions.is_cuda and turns.is_cuda and axis.is_cuda):
+        _need_cuda(positions, turns, axis)
+    dt = positions.dtype
+    if dt is not torch.int64 and dt is not torch.int32:
         raise ValueError(f"{what}: positions must be int32 or int64")
-    if positions.device != x.device or turns.device != x.device or axis.device != x.device:
+    dev = x.device
+    if positions.device != dev or turns.device != dev or axis.device != dev:
         raise ValueError(f"{what}: positions and the rotary table must be on the tensors' device")
-    if turns.dtype != torch.int64 or axis.dtype != torch.int32 or turns.shape != axis.shape or turns.ndim != 1 \
+    turned = turns.numel()
+    if turns.dtype is not torch.int64 or axis.dtype is not torch.int32 or turns.ndim != 1 or axis.shape != turns.shape \
             or not turns.is_contiguous() or not axis.is_contiguous():
         raise ValueError(f"{what}: the rotary table is an int64 and an int32 vector of one length")
-    if positions.ndim == 1 and axes == 1:
-        positions = positions.unsqueeze(-1)
-    batch, tokens = x.shape[:2]
-    if positions.ndim not in (2, 3) or positions.shape[-1] != axes or positions.shape[-2] != tokens \
-            or (positions.ndim == 3 and positions.shape[0] not in (1, batch)):
+    batch, tokens, _, dim = x.shape
+    shape, stride = positions.shape, positions.stride()
+    if len(shape) == 1 and axes == 1:
+        shape, stride = (shape[0], 1), (stride[0], 1)
+    if len(shape) not in (2, 3) or shape[-1] != axes or shape[-2] != tokens or (len(shape) == 3 and shape[0] != batch and shape[0] != 1):
         raise ValueError(f"{what}: positions must be [tokens, {axes}] or [batch, tokens, {axes}], got {tuple(positions.shape)} "
                          f"for {batch} x {tokens} tokens")
-    if 2 * turns.numel() > x.shape[3]:
-        raise ValueError(f"{what}: {turns.numel()} turning pairs do not fit head_dim {x.shape[3]}")
-    r.positions, r.positions_i64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-    r.stride_batch = positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0
-    r.stride_token, r.stride_axis = positions.stride(-2), positions.stride(-1)
-    r.axes, r.turned, r.interleaved = axes, turns.numel(), int(interleaved)
-    r.turns, r.axis = turns.data_ptr(), axis.data_ptr()
-    return r
+    if 2 * turned > dim:
+        raise ValueError(f"{what}: {turned} turning pairs do not fit head_dim {dim}")
+    return _lib.Rotary(positions.data_ptr(), int(dt is torch.int64), stride[0] if len(shape) == 3 and shape[0] > 1 else 0, stride[-2],
+                       stride[-1], axes, turned, int(interleaved), turns.data_ptr(), axis.data_ptr())
 
 
-def _check_heads(what, x):
-    for t in x:
-        _need_cuda(t)
-        if t.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"{what} runs on float32 / bfloat16 tensors")
-    x = _heads_args(what, x)
-    if x[0].shape[3] % 2 or not 2 <= x[0].shape[3] <= 512:
-        raise ValueError(f"{what} needs an even head_dim of 2 to 512, got {x[0].shape[3]}")
-    return x
+def _head_dim(what, dim):
+    if dim % 2 or not 2 <= dim <= 512:
+        raise ValueError(f"{what} needs an even head_dim of 2 to 512, got {dim}")
 
 
 def rotary(x, positions, table, inverse=False):
     """Rotates one or two [batch, tokens, heads, head_dim] tensors (any strides) by the positions'
     angles (the other way round with inverse=True); -> list of contiguous tensors.
     positions: int32 / int64 [tokens, axes] or [batch, tokens, axes]; table as in RotaryPositions.table."""
-    x = _check_heads("rotary", x)
-    dev = x[0].device
-    r = _rotary_args("rotary", x[0], positions, table)
-    with _on_device(dev):
-        y = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in x]
-        B, L, _, D = x[0].shape
-        rc = _lib.lib().fp4t_rotary(_heads_array(x), _heads_array(y), len(x), _lib.dtype_code(x[0].dtype), B, L, D,
-                                    ctypes.byref(r), int(inverse), _lib.stream_ptr(dev))
+    x, f = _heads("rotary", x)
+    t = x[0]
+    B, L, _, D = t.shape
+    _head_dim("rotary", D)
+    r = _rotary_args("rotary", t, positions, table)
+    dev, n = t.get_device(), len(x)
+    with _device_context(dev):
+        y = _outputs(x, f)
+        arr = _HEADS[2 * n](*f)
+        at = ctypes.addressof(arr)
+        rc = _lib.lib().fp4t_rotary(at, at + 40 * n, n, t.dtype is torch.float32, B, L, D, ctypes.addressof(r), inverse,
+                                    torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
         _lib.check(rc, "fp4t_rotary")
-        LAUNCHES["rotary"] += 1
+    LAUNCHES["rotary"] += 1
     return y
 
 
 def _qk_weights(what, x, weights):
     out = []
     for t, w in zip(x, weights):
-        if w.shape != (t.shape[3],) or w.device != t.device:
+        if w.ndim != 1 or w.shape[0] != t.shape[3] or w.device != t.device:
             raise ValueError(f"{what}: weights must be [head_dim] vectors on the tensors' device")
-        w = w.detach().to(torch.float32).contiguous()
-        out.append(w if w.data_ptr() % 16 == 0 else w.clone())
+        if w.dtype is not torch.float32 or not w.is_contiguous() or w.data_ptr() % 16:
+            w = w.detach().to(torch.float32).contiguous()
+            w = w if w.data_ptr() % 16 == 0 else w.clone()
+        out.append(w)
     return out
 
 
@@ -633,44 +670,55 @@ def _pointers(tensors):
 def qk_norm_rotary_forward(x, weights, eps, positions=None, table=None):
     """RMS norm of every head of one or two [batch, tokens, heads, head_dim] tensors, times its
     tensor's weight [head_dim], then the rotation of `rotary` (none without a table); statistics in fp32."""
-    x = _check_heads("qk_norm_rotary", x)
-    dev = x[0].device
-    r = _rotary_args("qk_norm_rotary", x[0], positions, table)
-    with _on_device(dev):
+    x, f = _heads("qk_norm_rotary", x)
+    t = x[0]
+    B, L, _, D = t.shape
+    _head_dim("qk_norm_rotary", D)
+    r = _rotary_args("qk_norm_rotary", t, positions, table)
+    dev, n = t.get_device(), len(x)
+    with _device_context(dev):
         w = _qk_weights("qk_norm_rotary", x, weights)
-        y = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in x]
-        B, L, _, D = x[0].shape
-        rc = _lib.lib().fp4t_qk_norm_rotary_forward(_heads_array(x), _pointers(w), float(eps), _heads_array(y), len(x),
-                                                    _lib.dtype_code(x[0].dtype), B, L, D, ctypes.byref(r), _lib.stream_ptr(dev))
+        y = _outputs(x, f)
+        arr = _HEADS[2 * n](*f)
+        at = ctypes.addressof(arr)
+        rc = _lib.lib().fp4t_qk_norm_rotary_forward(at, _pointers(w), eps, at + 40 * n, n, t.dtype is torch.float32, B, L, D,
+                                                    ctypes.addressof(r), torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
         _lib.check(rc, "fp4t_qk_norm_rotary_forward")
-        LAUNCHES["rotary"] += 1
+    LAUNCHES["rotary"] += 1
     return y
 
 
 def qk_norm_rotary_backward(dy, x, weights, eps, positions=None, table=None):
     """-> (list of dx like x, list of fp32 weight gradients [head_dim]) for the forward above."""
-    x = _check_heads("qk_norm_rotary", x)
-    dev = x[0].device
-    _need_cuda(*dy)
-    dy = _heads_args("qk_norm_rotary", [g.to(t.dtype) for g, t in zip(dy, x)], x[0])
-    if [g.shape for g in dy] != [t.shape for t in x]:
+    x, f = _heads("qk_norm_rotary", x)
+    t = x[0]
+    B, L, _, D = t.shape
+    _head_dim("qk_norm_rotary", D)
+    if any(g.dtype is not t.dtype for g in dy):
+        _need_cuda(*dy)
+        dy = [g.to(t.dtype) for g in dy]
+    dy, fg = _heads("qk_norm_rotary", dy, like=t)
+    if any(g.shape != s.shape for g, s in zip(dy, x)):
         raise ValueError("dy must have the shapes of x")
-    r = _rotary_args("qk_norm_rotary", x[0], positions, table)
-    with _on_device(dev):
-        L = _lib.lib()
+    r = _rotary_args("qk_norm_rotary", t, positions, table)
+    dev, n = t.get_device(), len(x)
+    with _device_context(dev):
+        lib = _lib.lib()
         w = _qk_weights("qk_norm_rotary", x, weights)
-        dx = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in x]
-        B, T, _, D = x[0].shape
-        dw = [torch.empty(D, dtype=torch.float32, device=dev) for _ in x]
-        ws_bytes = L.fp4t_qk_norm_rotary_backward_workspace_bytes(D)
+        dx = _outputs(x, f)
+        arr = _HEADS[3 * n](*f, *fg)
+        at = ctypes.addressof(arr)
+        ws_bytes = lib.fp4t_qk_norm_rotary_backward_workspace_bytes(D)
         if ws_bytes < 0:
             raise RuntimeError("fp4t_qk_norm_rotary_backward_workspace_bytes: unsupported shape or device")
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        rc = L.fp4t_qk_norm_rotary_backward(_heads_array(dy), _heads_array(x), _pointers(w), float(eps), _heads_array(dx),
-                                            _pointers(dw), len(x), _lib.dtype_code(x[0].dtype), B, T, D, ctypes.byref(r),
-                                            ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+        dw = [torch.empty(D, dtype=torch.float32, device=t.device) for _ in x]
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=t.device)
+        rc = lib.fp4t_qk_norm_rotary_backward(at + 80 * n, at, _pointers(w), eps, at + 40 * n, _pointers(dw), n, t.dtype is torch.float32,
+                                              B, L, D, ctypes.addressof(r), ws.data_ptr(), ws_bytes, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
         _lib.check(rc, "fp4t_qk_norm_rotary_backward")
-        LAUNCHES["rotary"] += 2
+    LAUNCHES["rotary"] += 2
     return dx, dw
 
 

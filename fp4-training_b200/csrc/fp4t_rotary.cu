@@ -8,14 +8,15 @@
 //
 // The angle is kept in turns as a 64-bit fixed-point fraction: position * (frequency / 2 pi * 2^64)
 // wraps modulo one turn by itself, so a position of a million is as exact as one of ten (an fp32
-// product is off by 0.06 radians there) and costs one integer multiply, no fp64.  Cosine and sine of a
-// (token, pair) are computed once per tile of tokens into shared memory and used by all heads of
-// queries AND keys of the token; with 3 + 3 heads the trigonometry is a third of the instructions,
-// with 32 + 8 it disappears.
+// product is off by 0.06 radians there) and costs one integer multiply, no fp64.
 //
 // A head is held by a group of 1 to 32 lanes, up to eight pairs (two 16-byte vectors of bf16) a lane, so the
 // norm is a shuffle reduction inside the group and every element is read and written once:
-// HBM-bound (forward 4 bytes per bf16 element, norm backward 6).
+// HBM-bound (forward 4 bytes per bf16 element, norm backward 6).  A group walks heads of ONE token,
+// queries and keys, with the cosines and sines of its pairs in registers: no shared memory, no barrier, and
+// the trigonometry is paid once per token, not per head.  Several heads' vectors are loaded before the
+// first is worked on, the first ones before the angles are computed.  Where tokens are few, a token's
+// heads are dealt out to several groups.
 #include <algorithm>
 
 #include "fp4t_common.cuh"
@@ -25,10 +26,8 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
-constexpr int kRotMaxTile = 32;           // tokens per tile
 constexpr int kRotMaxDim = 512;           // 256 pairs: 32 lanes x 8
-constexpr int kRotTableBytes = 32768;     // cosines and sines of one tile
-constexpr int kRotBlocksPerSm = 4;        // upper bound of the backward grid per SM (workspace size)
+constexpr int kRotBlocksPerSm = 2;        // of the norm backward: resident at once, and rows of its workspace
 
 struct HeadsIn {
   const void* p;
@@ -47,51 +46,52 @@ struct RotParams {
   int64_t n;                              // batch * tokens
   int64_t tokens;
   int dim, pairs, turned, group, log_group;
-  int tile;                               // tokens per tile
+  int chunk, chunks;                      // heads of a token per group, groups per token
+  int blocks0;                            // norm backward: blocks that work on the first tensor
   const void* pos;
   int pos_i64, axes;
   int64_t pos_sb, pos_st, pos_sa;
   const uint64_t* turns;
   const int32_t* axis;
   float sign;                             // -1: rotate back
-  float* partial;                         // norm backward: [gridDim.x][2][dim]
+  float* partial;                         // norm backward: [gridDim.x][dim]
 };
 
+// One vector of V elements as it lies in memory (bf16 stays packed until its head's turn comes: several
+// heads in flight fit the registers).
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float* v) {
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (V >= 4) {
+struct Raw {
+  static constexpr int kWords = sizeof(T) == 4 ? V : (V + 1) / 2;
+  uint32_t u[kWords];
+
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWords >= 4) {
 #pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(p + i);
-        v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 q = reinterpret_cast<const uint4*>(p)[i / 4];
+        u[i] = q.x; u[i + 1] = q.y; u[i + 2] = q.z; u[i + 3] = q.w;
       }
-    } else if constexpr (V == 2) {
-      const float2 f = *reinterpret_cast<const float2*>(p);
-      v[0] = f.x; v[1] = f.y;
-    } else {
-      v[0] = *p;
-    }
-  } else if constexpr (V == 1) {
-    v[0] = __bfloat162float(*p);
-  } else {
-    uint32_t u[V / 2];
-    if constexpr (V == 8) {
-      const uint4 q = *reinterpret_cast<const uint4*>(p);
-      u[0] = q.x; u[1] = q.y; u[2] = q.z; u[3] = q.w;
-    } else if constexpr (V == 4) {
+    } else if constexpr (kWords == 2) {
       const uint2 q = *reinterpret_cast<const uint2*>(p);
       u[0] = q.x; u[1] = q.y;
-    } else {
+    } else if constexpr (sizeof(T) == 4 || V == 2) {
       u[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    } else {
+      u[0] = *reinterpret_cast<const uint16_t*>(p);
     }
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) u[i] = 0u;
+  }
+  __device__ __forceinline__ void expand(float* v) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(u[i]);
+      else v[i] = __uint_as_float((i & 1) ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
+    }
+  }
+};
 
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float* v) {
@@ -132,30 +132,6 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t fraction) {
   return make_float2((quarter + 1u) & 2u ? -a : a, quarter & 2u ? -b : b);
 }
 
-// Index of pair p's cosine in a tile row: for eight-pair lanes the row is two halves, so that the
-// 16-byte reads of neighbouring lanes touch different banks.
-template <int V>
-__device__ __forceinline__ int table_index(int p, int turned) {
-  if constexpr (V == 8) return ((p >> 2) & 1) * (turned >> 1) + (p >> 3) * 4 + (p & 3);
-  else return p;
-}
-template <int V>
-__device__ __forceinline__ void load_table(const float* row, int p0, int turned, float* v) {
-  if constexpr (V == 8) {
-    const float4 a = *reinterpret_cast<const float4*>(row + (p0 >> 1));
-    const float4 b = *reinterpret_cast<const float4*>(row + (turned >> 1) + (p0 >> 1));
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else if constexpr (V == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(row + p0);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  } else if constexpr (V == 2) {
-    const float2 a = *reinterpret_cast<const float2*>(row + p0);
-    v[0] = a.x; v[1] = a.y;
-  } else {
-    v[0] = row[p0];
-  }
-}
-
 __device__ __forceinline__ float group_sum(float v, int group) {
   for (int o = group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
@@ -175,221 +151,292 @@ __device__ __forceinline__ void chunk_offsets(int p0, int turned, int& ea, int& 
   }
 }
 
-// Rotates the chunk in place by (cos, sin): e[0..V) and e[V..2V) are the two vectors.
-template <int V, bool kHalf>
-__device__ __forceinline__ void turn_chunk(float* e, const float* c, const float* s, float sign) {
+enum { kRotate = 0, kNormRotate = 1, kNormRotateBackward = 2 };
+
+// What a lane holds of a head: kSlots chunks of V pairs each (V * kSlots = 8 pairs), chunk s of lane j
+// starting at pair (j + s * group) * V.
+template <typename T, int V, bool kHalf>
+struct LaneView {
+  static constexpr int kSlots = 8 / V;
+  int ea[kSlots], eb[kSlots];      // element offsets of the chunk's two vectors
+  bool has[kSlots], turns[kSlots];
+
+  __device__ __forceinline__ void init(const RotParams& p, int lane) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int ia = kHalf ? i : 2 * i, ib = kHalf ? V + i : 2 * i + 1;
-    const float a = e[ia], b = e[ib], sn = s[i] * sign;
-    e[ia] = a * c[i] - b * sn;
-    e[ib] = a * sn + b * c[i];
+    for (int s = 0; s < kSlots; ++s) {
+      const int p0 = (lane + s * p.group) * V;
+      has[s] = p0 < p.pairs;
+      turns[s] = p0 < p.turned;
+      chunk_offsets<V, kHalf>(p0, p.turned, ea[s], eb[s]);
+    }
+  }
+  struct Head {
+    Raw<T, V> a[kSlots], b[kSlots];
+  };
+  __device__ __forceinline__ void load(const T* x, bool live, Head& r) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      if (live && has[s]) {
+        r.a[s].load(x + ea[s]);
+        r.b[s].load(x + eb[s]);
+      } else {
+        r.a[s].zero();
+        r.b[s].zero();
+      }
+    }
+  }
+  __device__ __forceinline__ void expand(const Head& r, float (&e)[16]) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      r.a[s].expand(e + 2 * V * s);
+      r.b[s].expand(e + 2 * V * s + V);
+    }
+  }
+  __device__ __forceinline__ void load_weight(const float* w, float (&e)[16]) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      Raw<float, V> a, b;
+      if (has[s]) {
+        a.load(w + ea[s]);
+        b.load(w + eb[s]);
+      } else {
+        a.zero();
+        b.zero();
+      }
+      a.expand(e + 2 * V * s);
+      b.expand(e + 2 * V * s + V);
+    }
+  }
+  __device__ __forceinline__ void store(T* y, const float (&e)[16]) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      if (has[s]) {
+        store_vec<T, V>(y + ea[s], e + 2 * V * s);
+        store_vec<T, V>(y + eb[s], e + 2 * V * s + V);
+      }
+    }
+  }
+  // cosines and sines (times sign) of the lane's pairs for the token at (b, l); 1 and 0 for those that stay
+  __device__ __forceinline__ void angles(const RotParams& p, int lane, int64_t b, int64_t l, float (&c)[8], float (&sn)[8]) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      const int p0 = (lane + s * p.group) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        c[V * s + i] = 1.f;
+        sn[V * s + i] = 0.f;
+      }
+      if (turns[s]) {
+        const int64_t at = b * p.pos_sb + l * p.pos_st;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const uint32_t a = min((uint32_t)__ldg(p.axis + p0 + i), (uint32_t)(p.axes - 1));   // never outside the positions
+          const int64_t j = at + (int64_t)a * p.pos_sa;
+          const int64_t pos = p.pos_i64 ? __ldg(static_cast<const long long*>(p.pos) + j) : (int64_t)__ldg(static_cast<const int*>(p.pos) + j);
+          const float2 cs = turn_cos_sin((uint64_t)pos * __ldg(reinterpret_cast<const unsigned long long*>(p.turns) + p0 + i));
+          c[V * s + i] = cs.x;
+          sn[V * s + i] = cs.y * p.sign;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void turn(float (&e)[16], const float (&c)[8], const float (&sn)[8], float sign) const {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      if (turns[s]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int ia = 2 * V * s + (kHalf ? i : 2 * i), ib = 2 * V * s + (kHalf ? V + i : 2 * i + 1);
+          const float a = e[ia], b = e[ib], k = c[V * s + i], t = sn[V * s + i] * sign;
+          e[ia] = a * k - b * t;
+          e[ib] = a * t + b * k;
+        }
+      }
+    }
+  }
+};
+
+// Forward (and the plain rotation's backward).  A warp works on 32 / group tokens and one chunk of
+// their heads; kBatch heads are in flight per lane.
+template <typename T, int V, bool kHalf, bool kNorm>
+__global__ void __launch_bounds__(kRotThreads, 2) qk_rotary_kernel(const RotParams p) {
+  constexpr int kBatch = sizeof(T) == 4 ? 2 : V == 1 ? 2 : 4;      // 32 registers of raw vectors
+  const int lane = threadIdx.x & (p.group - 1);
+  const int per_warp = 32 >> p.log_group;
+  const int64_t unit = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5);
+  const int64_t tb = unit / p.chunks;
+  const int chunk = (int)(unit - tb * p.chunks);
+  const int64_t n = tb * per_warp + ((threadIdx.x & 31) >> p.log_group);
+  if (tb * per_warp >= p.n) return;                       // the whole warp
+  const bool token_live = n < p.n;
+  const int64_t nn = token_live ? n : p.n - 1, b = nn / p.tokens, l = nn - b * p.tokens;
+  LaneView<T, V, kHalf> view;
+  view.init(p, lane);
+  float c[8], sn[8];
+  bool have_angles = false;
+  const int h0 = chunk * p.chunk, h1 = h0 + p.chunk;      // heads of the chunk, keys behind the queries
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int shift = which == 0 ? 0 : p.heads[0];
+    const int first = max(h0 - shift, 0), last = min(h1 - shift, p.heads[which]);
+    if (first >= last) continue;                          // warp-uniform
+    const T* x = static_cast<const T*>(p.x[which].p) + b * p.x[which].sb + l * p.x[which].st;
+    T* y = static_cast<T*>(p.y[which].p) + b * p.y[which].sb + l * p.y[which].st;
+    typename LaneView<T, V, kHalf>::Head raw[kBatch];
+    float w[16];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) view.load(x + (first + u) * p.x[which].sh, token_live && first + u < last, raw[u]);
+    if (!have_angles) {
+      view.angles(p, lane, b, l, c, sn);
+      have_angles = true;
+    }
+    if (kNorm) view.load_weight(p.w[which], w);
+    for (int h = first;;) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (h + u < last) {                               // warp-uniform
+          float e[16];
+          view.expand(raw[u], e);
+          if (kNorm) {
+            float sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sq = fmaf(e[i], e[i], sq);
+            const float r = rsqrtf(group_sum(sq, p.group) * p.inv_dim + p.eps);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) e[i] = (e[i] * r) * w[i];
+          }
+          view.turn(e, c, sn, 1.f);
+          if (token_live) view.store(y + (h + u) * p.y[which].sh, e);
+        }
+      }
+      h += kBatch;
+      if (h >= last) break;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) view.load(x + (h + u) * p.x[which].sh, token_live && h + u < last, raw[u]);
+    }
   }
 }
 
-enum { kRotate = 0, kNormRotate = 1, kNormRotateBackward = 2 };
-
-// V pairs per vector, kSlots vectors pairs per lane (V * kSlots = 8 pairs).
-template <typename T, int V, bool kHalf, int kMode>
-__global__ void __launch_bounds__(kRotThreads) qk_rotary_kernel(const RotParams p) {
-  constexpr int kSlots = 8 / V;
-  constexpr bool kNorm = kMode != kRotate, kBack = kMode == kNormRotateBackward;
-  extern __shared__ __align__(16) float table[];        // [tile][2][turned]; reused for the weight gradients
-  __shared__ int64_t off_x[2][kRotMaxTile], off_y[2][kRotMaxTile], off_g[2][kRotMaxTile];
-  const int lane_in_group = threadIdx.x & (p.group - 1);
-  const int first = threadIdx.x >> p.log_group, stride = kRotThreads >> p.log_group;
-  float dw[2][16];
-  if (kBack) {
+// Norm backward.  A block works on one of the tensors, so that a lane's weight gradients are 16 registers;
+// persistent: they are kept over all its tokens and reduced once.
+template <typename T, int V, bool kHalf>
+__global__ void __launch_bounds__(kRotThreads, 2) qk_norm_rotary_bwd_kernel(const RotParams p) {
+  constexpr int kBatch = sizeof(T) == 4 || V == 1 ? 1 : 2;         // 32 registers of raw vectors
+  __shared__ float red[kRotMaxDim];
+  const int which = (int)blockIdx.x < p.blocks0 ? 0 : 1;
+  const int block = which == 0 ? blockIdx.x : blockIdx.x - p.blocks0;
+  const int blocks = which == 0 ? p.blocks0 : gridDim.x - p.blocks0;
+  const HeadsIn px = p.x[which], pg = p.dy[which];
+  const HeadsOut py = p.y[which];
+  const int heads = p.heads[which];
+  const int lane = threadIdx.x & (p.group - 1), warp = threadIdx.x >> 5;
+  const int per_warp = 32 >> p.log_group;
+  LaneView<T, V, kHalf> view;
+  view.init(p, lane);
+  float w[16], dw[16];
+  view.load_weight(p.w[which], w);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0.f;
-  }
-  const int64_t tiles = (p.n + p.tile - 1) / p.tile;
-  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int64_t n0 = t * p.tile;
-    const int count = (int)min((int64_t)p.tile, p.n - n0);
-    __syncthreads();                                     // the previous tile's table is no longer read
-    if (threadIdx.x < count) {
-      const int64_t n = n0 + threadIdx.x, b = n / p.tokens, l = n - b * p.tokens;
+  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
+  const int chunks = (heads + p.chunk - 1) / p.chunk;
+  const int64_t units = (p.n + per_warp - 1) / per_warp * chunks;
+  for (int64_t unit = (int64_t)block * kRotWarps + warp; unit < units; unit += (int64_t)blocks * kRotWarps) {
+    const int64_t tb = unit / chunks;
+    const int first = (int)(unit - tb * chunks) * p.chunk, last = min(first + p.chunk, heads);
+    const int64_t n = tb * per_warp + ((threadIdx.x & 31) >> p.log_group);
+    const bool live = n < p.n;
+    const int64_t nn = live ? n : p.n - 1, b = nn / p.tokens, l = nn - b * p.tokens;
+    const T* x = static_cast<const T*>(px.p) + b * px.sb + l * px.st;
+    const T* g = static_cast<const T*>(pg.p) + b * pg.sb + l * pg.st;
+    T* y = static_cast<T*>(py.p) + b * py.sb + l * py.st;
+    typename LaneView<T, V, kHalf>::Head raw_x[kBatch], raw_g[kBatch];
+    float c[8], sn[8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        off_x[i][threadIdx.x] = b * p.x[i].sb + l * p.x[i].st;
-        off_y[i][threadIdx.x] = b * p.y[i].sb + l * p.y[i].st;
-        if (kBack) off_g[i][threadIdx.x] = b * p.dy[i].sb + l * p.dy[i].st;
-      }
+    for (int k = 0; k < kBatch; ++k) {
+      view.load(x + (first + k) * px.sh, live && first + k < last, raw_x[k]);
+      view.load(g + (first + k) * pg.sh, live && first + k < last, raw_g[k]);
     }
-    for (int i = threadIdx.x; i < count * p.turned; i += kRotThreads) {
-      const int tok = i / p.turned, pr = i - tok * p.turned;
-      const int64_t n = n0 + tok, b = n / p.tokens, l = n - b * p.tokens;
-      const uint32_t a = min((uint32_t)__ldg(p.axis + pr), (uint32_t)(p.axes - 1));   // never outside the positions
-      const int64_t at = b * p.pos_sb + l * p.pos_st + (int64_t)a * p.pos_sa;
-      const int64_t pos = p.pos_i64 ? __ldg(static_cast<const long long*>(p.pos) + at) : (int64_t)__ldg(static_cast<const int*>(p.pos) + at);
-      const float2 cs = turn_cos_sin((uint64_t)pos * __ldg(reinterpret_cast<const unsigned long long*>(p.turns) + pr));
-      const int j = table_index<V>(pr, p.turned);
-      table[(2 * tok) * p.turned + j] = cs.x;
-      table[(2 * tok + 1) * p.turned + j] = cs.y;
-    }
-    __syncthreads();
+    view.angles(p, lane, b, l, c, sn);
+    for (int h = first;;) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int heads = p.heads[which];
-      const int items = count * heads;
-      const T* x0 = static_cast<const T*>(p.x[which].p);
-      T* y0 = static_cast<T*>(p.y[which].p);
-      // all lanes of a warp take the same number of turns (shuffles); groups behind the last item idle
-      const int rounds = (items + stride - 1) / stride;
-      for (int it = 0; it < rounds; ++it) {
-        const int item = first + it * stride;
-        const bool live = item < items;
-        const int tok = live ? item / heads : 0, head = live ? item - tok * heads : 0;
-        const T* x = x0 + off_x[which][tok] + head * p.x[which].sh;
-        T* y = y0 + off_y[which][tok] + head * p.y[which].sh;
-        const float* crow = table + 2 * tok * p.turned;
-        const float* srow = crow + p.turned;
-        float e[kSlots][2 * V];
-        float sq = 0.f;
+      for (int k = 0; k < kBatch; ++k) {
+        if (h + k < last) {                               // warp-uniform; a dead token's vectors are zero
+          float e[16], u[16];
+          view.expand(raw_x[k], e);
+          view.expand(raw_g[k], u);
+          float sq = 0.f;
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s) {
-          const int p0 = (lane_in_group + s * p.group) * V;
-          if (live && p0 < p.pairs) {
-            int ea, eb;
-            chunk_offsets<V, kHalf>(p0, p.turned, ea, eb);
-            load_vec<T, V>(x + ea, e[s]);
-            load_vec<T, V>(x + eb, e[s] + V);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) e[s][i] = 0.f;
-          }
-          if (kNorm) {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) sq = fmaf(e[s][i], e[s][i], sq);
-          }
-        }
-        float r = 1.f;
-        if (kNorm) r = rsqrtf(group_sum(sq, p.group) * p.inv_dim + p.eps);
-        if (!kBack) {
-          if (!live) continue;                           // no shuffles below
-#pragma unroll
-          for (int s = 0; s < kSlots; ++s) {
-            const int p0 = (lane_in_group + s * p.group) * V;
-            if (p0 >= p.pairs) continue;
-            int ea, eb;
-            chunk_offsets<V, kHalf>(p0, p.turned, ea, eb);
-            if (kNorm) {
-              float w[2 * V];
-              load_vec<float, V>(p.w[which] + ea, w);
-              load_vec<float, V>(p.w[which] + eb, w + V);
-#pragma unroll
-              for (int i = 0; i < 2 * V; ++i) e[s][i] = (e[s][i] * r) * w[i];
-            }
-            if (p0 < p.turned) {
-              float c[V], sn[V];
-              load_table<V>(crow, p0, p.turned, c);
-              load_table<V>(srow, p0, p.turned, sn);
-              turn_chunk<V, kHalf>(e[s], c, sn, p.sign);
-            }
-            store_vec<T, V>(y + ea, e[s]);
-            store_vec<T, V>(y + eb, e[s] + V);
-          }
-        } else {
-          const T* dy = static_cast<const T*>(p.dy[which].p) + off_g[which][tok] + head * p.dy[which].sh;
-          float u[kSlots][2 * V];
+          for (int i = 0; i < 16; ++i) sq = fmaf(e[i], e[i], sq);
+          const float r = rsqrtf(group_sum(sq, p.group) * p.inv_dim + p.eps);
+          view.turn(u, c, sn, -1.f);
           float dot = 0.f;
+          if (live) {                                     // (a dead token's r may be infinite)
 #pragma unroll
-          for (int s = 0; s < kSlots; ++s) {
-            const int p0 = (lane_in_group + s * p.group) * V;
-            if (live && p0 < p.pairs) {
-              int ea, eb;
-              chunk_offsets<V, kHalf>(p0, p.turned, ea, eb);
-              load_vec<T, V>(dy + ea, u[s]);
-              load_vec<T, V>(dy + eb, u[s] + V);
-              if (p0 < p.turned) {
-                float c[V], sn[V];
-                load_table<V>(crow, p0, p.turned, c);
-                load_table<V>(srow, p0, p.turned, sn);
-                turn_chunk<V, kHalf>(u[s], c, sn, -1.f);
-              }
-              float w[2 * V];
-              load_vec<float, V>(p.w[which] + ea, w);
-              load_vec<float, V>(p.w[which] + eb, w + V);
-#pragma unroll
-              for (int i = 0; i < 2 * V; ++i) {
-                e[s][i] *= r;                                               // xh
-                dw[which][s * 2 * V + i] = fmaf(u[s][i], e[s][i], dw[which][s * 2 * V + i]);
-                u[s][i] *= w[i];
-                dot = fmaf(u[s][i], e[s][i], dot);
-              }
+            for (int i = 0; i < 16; ++i) {
+              e[i] *= r;                               // xh
+              dw[i] = fmaf(u[i], e[i], dw[i]);
+              u[i] *= w[i];
+              dot = fmaf(u[i], e[i], dot);
             }
           }
           dot = group_sum(dot, p.group) * p.inv_dim;
-          if (!live) continue;
+          if (live) {
 #pragma unroll
-          for (int s = 0; s < kSlots; ++s) {
-            const int p0 = (lane_in_group + s * p.group) * V;
-            if (p0 >= p.pairs) continue;
-            int ea, eb;
-            chunk_offsets<V, kHalf>(p0, p.turned, ea, eb);
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) u[s][i] = r * (u[s][i] - e[s][i] * dot);
-            store_vec<T, V>(y + ea, u[s]);
-            store_vec<T, V>(y + eb, u[s] + V);
+            for (int i = 0; i < 16; ++i) u[i] = r * (u[i] - e[i] * dot);
+            view.store(y + (h + k) * py.sh, u);
           }
         }
       }
+      h += kBatch;
+      if (h >= last) break;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        view.load(x + (h + k) * px.sh, live && h + k < last, raw_x[k]);
+        view.load(g + (h + k) * pg.sh, live && h + k < last, raw_g[k]);
+      }
     }
   }
-  if (kBack) {
-    // The block's weight gradients: the groups of a warp by shuffles, the warps in warp order, then one
-    // row of the workspace -- a fixed association, whatever the scheduling.
-    float* red = table;                                  // [2][dim]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // The block's weight gradients: the groups of a warp by shuffles, the warps in warp order, then one
+  // row of the workspace -- a fixed association, whatever the scheduling.
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
+  for (int i = 0; i < 16; ++i)
+    for (int o = p.group; o < 32; o <<= 1) dw[i] += __shfl_xor_sync(0xFFFFFFFFu, dw[i], o);
+  for (int wi = 0; wi < kRotWarps; ++wi) {
+    if (warp == wi && (threadIdx.x & 31) < p.group) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        for (int o = p.group; o < 32; o <<= 1) dw[which][i] += __shfl_xor_sync(0xFFFFFFFFu, dw[which][i], o);
-    }
-    for (int wi = 0; wi < kRotWarps; ++wi) {
-      __syncthreads();
-      if (warp == wi && lane < p.group) {
+      for (int s = 0; s < view.kSlots; ++s) {
+        if (view.has[s]) {
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-#pragma unroll
-          for (int s = 0; s < kSlots; ++s) {
-            const int p0 = (lane + s * p.group) * V;
-            if (p0 >= p.pairs) continue;
-            int ea, eb;
-            chunk_offsets<V, kHalf>(p0, p.turned, ea, eb);
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) {
-              float* at = red + which * p.dim + (i < V ? ea + i : eb + i - V);
-              *at = wi == 0 ? dw[which][s * 2 * V + i] : *at + dw[which][s * 2 * V + i];
-            }
+          for (int i = 0; i < 2 * V; ++i) {
+            float* at = red + (i < V ? view.ea[s] + i : view.eb[s] + i - V);
+            *at = wi == 0 ? dw[2 * V * s + i] : *at + dw[2 * V * s + i];
           }
         }
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * p.dim; i += kRotThreads) p.partial[(size_t)blockIdx.x * 2 * p.dim + i] = red[i];
   }
+  for (int i = threadIdx.x; i < p.dim; i += kRotThreads) p.partial[(size_t)blockIdx.x * p.dim + i] = red[i];
 }
 
-// dweight[c] = sum over the blocks' partial rows, in a fixed order: one block per 32 columns, warp w adds
-// rows w, w + 32, ..., then the warps' sums are added in warp order.
-__global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const float* __restrict__ partial, int parts, int dim,
+// dweight[c] = sum over a tensor's blocks' partial rows, in a fixed order: one block per 32 columns of a
+// tensor, warp w adds rows w, w + 32, ..., then the warps' sums are added in warp order.
+__global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const float* __restrict__ partial, int blocks0, int blocks, int dim,
                                                               float* __restrict__ dq, float* __restrict__ dk) {
   __shared__ float red[32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int i = blockIdx.x * 32 + lane;
+  const int from = blockIdx.y == 0 ? 0 : blocks0, to = blockIdx.y == 0 ? blocks0 : blocks;
   float s = 0.f;
-  if (i < 2 * dim)
-    for (int k = warp; k < parts; k += 32) s += partial[(size_t)k * 2 * dim + i];
+  if (i < dim) {
+#pragma unroll 8
+    for (int k = from + warp; k < to; k += 32) s += partial[(size_t)k * dim + i];
+  }
   red[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && i < 2 * dim) {
+  if (warp == 0 && i < dim) {
     float v = 0.f;
     for (int w = 0; w < 32; ++w) v += red[w][lane];
-    if (i < dim) dq[i] = v;
-    else if (dk != nullptr) dk[i - dim] = v;
+    (blockIdx.y == 0 ? dq : dk)[i] = v;
   }
 }
 
@@ -397,8 +444,8 @@ using RotKernel = void (*)(const RotParams);
 
 template <typename T, int V, bool kHalf>
 RotKernel pick_mode(int mode) {
-  return mode == kRotate ? qk_rotary_kernel<T, V, kHalf, kRotate>
-         : mode == kNormRotate ? qk_rotary_kernel<T, V, kHalf, kNormRotate> : qk_rotary_kernel<T, V, kHalf, kNormRotateBackward>;
+  return mode == kRotate ? qk_rotary_kernel<T, V, kHalf, false>
+         : mode == kNormRotate ? qk_rotary_kernel<T, V, kHalf, true> : qk_norm_rotary_bwd_kernel<T, V, kHalf>;
 }
 template <typename T, int V>
 RotKernel pick_layout(bool half, int mode) {
@@ -461,9 +508,9 @@ int run(const char* name, int mode, const fp4t_heads_t* x, const fp4t_heads_t* d
                "%s: a tensor is not aligned to its elements", name);
   if (norm) FP4T_REQUIRE(eps >= 0.0f, "%s: eps must not be negative", name);
   if (mode == kNormRotateBackward) FP4T_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be 16-byte aligned", name);
-  const int64_t row_bytes = 2 * dim * (int64_t)sizeof(float);    // of the workspace: one row per block
-  if (mode == kNormRotateBackward) FP4T_REQUIRE(workspace_bytes >= row_bytes, "%s: the workspace holds %lld bytes, %lld are the least", name,
-                                                (long long)workspace_bytes, (long long)row_bytes);
+  const int64_t row_bytes = dim * (int64_t)sizeof(float);        // of the workspace: one row per block
+  if (mode == kNormRotateBackward) FP4T_REQUIRE(workspace_bytes >= count * row_bytes, "%s: the workspace holds %lld bytes, %lld are the least", name,
+                                                (long long)workspace_bytes, (long long)(count * row_bytes));
   if (empty) {
     if (mode == kNormRotateBackward)
       for (int i = 0; i < count; ++i) FP4T_CUDA(cudaMemsetAsync(dw[i], 0, (size_t)dim * sizeof(float), stream));
@@ -514,32 +561,42 @@ int run(const char* name, int mode, const fp4t_heads_t* x, const fp4t_heads_t* d
     p.group <<= 1;
     ++p.log_group;
   }
-  // Tokens per tile: enough items for two rounds of all groups, a table of at most 32 KB, and no
-  // fewer tiles than SMs while there are tokens to spread.
-  const int per_round = kRotThreads >> p.log_group, heads = p.heads[0] + p.heads[1];
-  int64_t tile = std::max<int64_t>(1, (2 * per_round + heads - 1) / heads);
-  tile = std::max<int64_t>(tile, 4);
-  tile = std::min<int64_t>(tile, kRotMaxTile);
-  if (p.turned > 0) tile = std::min<int64_t>(tile, kRotTableBytes / (8 * p.turned));
-  tile = std::min<int64_t>(tile, std::max<int64_t>(1, p.n / (2 * sms)));
-  p.tile = (int)tile;
+  // A token's heads go to one group unless that leaves warps short of eight per SM (about the number that
+  // hides the loads' latency); then they are dealt out, down to one head per group.
+  const int per_warp = 32 >> p.log_group;
+  const int64_t token_warps = ceil_div(p.n, per_warp), enough = 8ll * sms;
+  const auto chunk_for = [&](int heads) {
+    const int64_t chunks = std::min<int64_t>(heads, std::max<int64_t>(1, enough / token_warps));
+    return (int)ceil_div(heads, chunks);
+  };
   RotKernel kern = dtype == FP4T_DT_F32 ? pick_width<float>(v, half, mode) : pick_width<__nv_bfloat16>(v, half, mode);
-  const size_t smem = std::max((size_t)tile * 2 * p.turned * 4, mode == kNormRotateBackward ? (size_t)2 * dim * 4 : (size_t)0);
-  int occ = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kRotThreads, smem) != cudaSuccess || occ <= 0) {
-    cudaGetLastError();
-    occ = 1;
-  }
-  if (mode == kNormRotateBackward) occ = std::min(occ, kRotBlocksPerSm);
-  const int64_t tiles = ceil_div(p.n, tile);
-  int grid = (int)std::min<int64_t>(tiles, (int64_t)sms * occ);
-  if (mode == kNormRotateBackward) grid = (int)std::min<int64_t>(grid, workspace_bytes / row_bytes);
-  kern<<<grid, kRotThreads, smem, stream>>>(p);
-  FP4T_CUDA(cudaGetLastError());
-  if (mode == kNormRotateBackward) {
-    qk_weight_grad_kernel<<<(int)ceil_div(2 * dim, 32), 1024, 0, stream>>>(p.partial, grid, (int)dim, dw[0], count == 2 ? dw[1] : nullptr);
+  if (mode != kNormRotateBackward) {
+    const int heads = p.heads[0] + p.heads[1];
+    p.chunk = chunk_for(heads);
+    p.chunks = (int)ceil_div(heads, p.chunk);
+    const int64_t blocks = ceil_div(token_warps * p.chunks, kRotWarps);
+    FP4T_REQUIRE(blocks <= INT32_MAX, "%s: too many tokens", name);
+    kern<<<(unsigned)blocks, kRotThreads, 0, stream>>>(p);
     FP4T_CUDA(cudaGetLastError());
+    return FP4T_OK;
   }
+  // Persistent blocks, two per SM, dealt out to the tensors by their heads; no more than there is work or
+  // workspace for.
+  p.chunk = chunk_for(std::max(p.heads[0], p.heads[1]));
+  const auto blocks_for = [&](int heads) { return std::max<int64_t>(1, ceil_div(token_warps * ceil_div(heads, p.chunk), kRotWarps)); };
+  const int64_t room = std::min<int64_t>((int64_t)kRotBlocksPerSm * sms, workspace_bytes / row_bytes);
+  int64_t b0 = blocks_for(p.heads[0]), b1 = count == 2 ? blocks_for(p.heads[1]) : 0;
+  if (b0 + b1 > room) {
+    const int64_t share = b1 == 0 ? room : std::max<int64_t>(1, std::min<int64_t>(room - 1, room * p.heads[0] / (p.heads[0] + p.heads[1])));
+    b0 = std::min(b0, share);
+    b1 = std::min(b1, room - share);
+  }
+  p.blocks0 = (int)b0;
+  kern<<<(unsigned)(b0 + b1), kRotThreads, 0, stream>>>(p);
+  FP4T_CUDA(cudaGetLastError());
+  qk_weight_grad_kernel<<<dim3((unsigned)ceil_div(dim, 32), (unsigned)count), 1024, 0, stream>>>(p.partial, (int)b0, (int)(b0 + b1), (int)dim,
+                                                                                                dw[0], count == 2 ? dw[1] : nullptr);
+  FP4T_CUDA(cudaGetLastError());
   return FP4T_OK;
 }
 
@@ -564,7 +621,7 @@ extern "C" int fp4t_qk_norm_rotary_forward(const fp4t_heads_t* x, const float* c
 extern "C" int64_t fp4t_qk_norm_rotary_backward_workspace_bytes(int64_t head_dim) {
   const int sms = sm_count();
   if (head_dim < 2 || head_dim > kRotMaxDim || sms <= 0) return -1;
-  return (int64_t)sms * kRotBlocksPerSm * 2 * head_dim * (int64_t)sizeof(float);
+  return (int64_t)sms * kRotBlocksPerSm * head_dim * (int64_t)sizeof(float);
 }
 
 extern "C" int fp4t_qk_norm_rotary_backward(const fp4t_heads_t* dy, const fp4t_heads_t* x, const float* const* weights, float eps,

@@ -51,11 +51,19 @@ class _QKNormFn(torch.autograd.Function):
         x, w = args[:ctx.count], args[ctx.count:]
         table = None if ctx.table is None else (turns, axis) + ctx.table
         dx, dw = _ops.qk_norm_rotary_backward(dy, x, w, ctx.eps, positions, table)
-        return (None, None, None, None, *dx, *[g.to(t.dtype) for g, t in zip(dw, w)])
+        return (None, None, None, None, *dx, *[g if t.dtype is torch.float32 else g.to(t.dtype) for g, t in zip(dw, w)])
 
 
-def _with_batch(x):
-    return [t.unsqueeze(0) if t.ndim == 3 else t for t in x]
+def _rotate(positions, table, *x):
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in x)):
+        return _ops.rotary(x, positions, table)
+    return _RotaryFn.apply(positions, table, *x)
+
+
+def _qk_norm(positions, table, eps, q, k, wq, wk):
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or wq.requires_grad or wk.requires_grad)):
+        return _ops.qk_norm_rotary_forward((q, k), (wq, wk), eps, positions, table)
+    return _QKNormFn.apply(positions, table, eps, 2, q, k, wq, wk)
 
 
 class RotaryPositions(nn.Module):
@@ -111,7 +119,8 @@ class RotaryPositions(nn.Module):
 
     @property
     def table(self):
-        return self.turns, self.axis, len(self.sections), self.layout == "interleaved"
+        buffers = self._buffers
+        return buffers["turns"], buffers["axis"], len(self.sections), self.layout == "interleaved"
 
     def _check(self, x):
         if x[0].shape[-1] != self.head_dim:
@@ -122,9 +131,11 @@ class RotaryPositions(nn.Module):
         if len(x) not in (1, 2):
             raise ValueError("RotaryPositions takes one or two tensors")
         self._check(x)
-        y = _RotaryFn.apply(positions, self.table, *_with_batch(x))
-        y = tuple(o.view(t.shape) for o, t in zip(y, x))
-        return y if len(y) == 2 else y[0]
+        if x[0].ndim == 3:
+            y = [o.squeeze(0) for o in _rotate(positions, self.table, *[t.unsqueeze(0) for t in x])]
+        else:
+            y = _rotate(positions, self.table, *x)
+        return tuple(y) if len(x) == 2 else y[0]
 
     def extra_repr(self):
         return f"head_dim={self.head_dim}, sections={self.sections}, layout={self.layout!r}"
@@ -151,9 +162,10 @@ class FusedQKNorm(nn.Module):
         if q.shape[-1] != self.head_dim:
             raise ValueError(f"head_dim {q.shape[-1]} is not this module's {self.head_dim}")
         table = None if self.rotary is None else self.rotary.table
-        x = _with_batch((q, k))
-        qo, ko = _QKNormFn.apply(positions, table, self.eps, 2, *x, self.q_weight, self.k_weight)
-        return qo.view(q.shape), ko.view(k.shape)
+        if q.ndim == 3:
+            qo, ko = _qk_norm(positions, table, self.eps, q.unsqueeze(0), k.unsqueeze(0), self.q_weight, self.k_weight)
+            return qo.squeeze(0), ko.squeeze(0)
+        return tuple(_qk_norm(positions, table, self.eps, q, k, self.q_weight, self.k_weight))
 
     def extra_repr(self):
         return f"head_dim={self.head_dim}, eps={self.eps}"

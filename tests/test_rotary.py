@@ -56,10 +56,7 @@ def test_argument_errors_of_the_c_entries():
     buf = 0x10000
 
     def heads(n=2, data=buf, h=3, st=(192, 192, 64)):
-        arr = (_lib.Heads * n)()
-        for a in arr:
-            a.data, a.heads, a.stride_batch, a.stride_token, a.stride_head = data, h, *st
-        return arr
+        return (ctypes.c_int64 * (5 * n))(*([data or 0, h, *st] * n))
 
     def rotary(turned=8, axes=2, positions=buf, turns=buf, axis=buf):
         r = _lib.Rotary()

@@ -59,6 +59,7 @@ struct XParams {
   const int* slots;                              // number of counted tokens
   int tokens;                                    // all tokens: slots == tokens means that h can be read as it is
   int slot0;                                     // kStats: first slot of the block
+  int split_clusters;                            // kProduct: clusters that K may be split over (0: it may not)
   // kStats, kGrad
   const void* bias;
   int bias_f32;
@@ -125,6 +126,25 @@ template <bool kMn>
 __device__ __forceinline__ uint64_t xent_desc(uint32_t lo, int k16) {
   return kMn ? make_desc((lo + (uint32_t)k16 * (2048u >> 4)) | kMnLead, kDescHiOperand)
              : make_desc(lo + (uint32_t)k16 * (32u >> 4), kDescHiOperand);
+}
+
+// kProduct's K splits follow the number of slots too: over the clusters that its tiles leave idle, if those
+// are at least half, into pieces of two stages or more.  splits * m_tiles * n_tiles <= clusters, which
+// bounds the slices.
+struct SlotSplit {
+  int splits, ks_per_split;
+};
+__host__ __device__ __forceinline__ SlotSplit split_slots(int m_tiles, int n_tiles, int k_stages, int clusters) {
+  const int tiles = m_tiles * n_tiles;
+  SlotSplit r{1, k_stages};
+  if (tiles > 0 && (int64_t)m_tiles * n_tiles * 2 <= clusters && k_stages >= 4) {
+    const int s = min(clusters / tiles, k_stages / 2);
+    if (s >= 2) {
+      r.ks_per_split = (k_stages + s - 1) / s;
+      r.splits = (k_stages + r.ks_per_split - 1) / r.ks_per_split;
+    }
+  }
+  return r;
 }
 
 struct TilePos {
@@ -286,7 +306,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   if (threadIdx.x == 32) {
     tma_prefetch_map(&map_a);
     tma_prefetch_map(&map_b);
-    if (kMode != kProduct) tma_prefetch_map(&map_packed);
+    if (kMode != kProduct || gp.split_clusters > 0) tma_prefetch_map(&map_packed);
     if (kMode != kStats) tma_prefetch_map(&map_d);
   }
   if (threadIdx.x == 0) {
@@ -322,7 +342,14 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   } else {
     g.rows = max(0, min(g.rows, slots - g.slot0));
     g.m_tiles = (g.rows + kXM - 1) / kXM;
+    if (kMode == kProduct && g.split_clusters > 0) {
+      const SlotSplit sp = split_slots(g.m_tiles, g.n_tiles, g.k_stages, g.split_clusters);
+      g.splits = sp.splits;
+      g.ks_per_split = sp.ks_per_split;
+      g.slice_rows = g.m_tiles * kXM;
+    }
   }
+  const bool sliced = kMode == kProduct && g.splits > 1;      // fp32 slices (map_packed), summed by another kernel
   const CUtensorMap* tma_a = (kMode == kStats || kMode == kGrad) && !dense ? &map_packed : &map_a;
   const CUtensorMap* tma_b = kMode == kProductT && !dense ? &map_packed : &map_b;
   const int units = g.m_tiles * g.n_tiles * g.splits;
@@ -530,7 +557,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = nothing ? 0.f : __uint_as_float(r[j]);
-          if (g.acc != nullptr && row_ok) {                    // columns are a multiple of 8: whole vectors
+          if (g.acc != nullptr && row_ok && !sliced) {         // columns are a multiple of 8: whole vectors
             const float4* p = reinterpret_cast<const float4*>(g.acc + (int64_t)row * g.ldacc + col);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -541,7 +568,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
           }
           const int srow = row0 + t.split * g.slice_rows;
-          if (kMode == kProduct && g.out != nullptr && !dense) store_row_chunk(out_row, g.out_f32, col, g.cols, v);
+          if (sliced) store_chunk_f32(&map_packed, buf, lane, srow, col, v);
+          else if (kMode == kProduct && g.out != nullptr && !dense) store_row_chunk(out_row, g.out_f32, col, g.cols, v);
           else if (g.out_f32) store_chunk_f32(&map_d, buf, lane, srow, col, v);
           else store_chunk_bf16(&map_d, buf, n_emit, lane, srow, col, v);
         }
@@ -621,6 +649,7 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
       if (i < (int)blockIdx.x) before += c;
     }
   } else {
+#pragma unroll 8
     for (int t = threadIdx.x; t < p.tokens; t += kPackThreads) {
       const int c = __ldg(reinterpret_cast<const long long*>(p.target) + t) != p.ignore;
       all += c;
@@ -661,7 +690,15 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
       for (int i = warp; i < total; i += kPackThreads / 32) {
         const uint4* from = reinterpret_cast<const uint4*>(p.h + (int64_t)source[i] * p.ldh);
         uint4* to = reinterpret_cast<uint4*>(p.packed + (int64_t)(before + i) * p.dim);
-        for (int c = lane; c < p.dim / 8; c += 32) to[c] = from[c];
+        for (int c0 = lane; c0 < p.dim / 8; c0 += 128) {
+          uint4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c0 + 32 * k < p.dim / 8) v[k] = __ldg(from + c0 + 32 * k);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c0 + 32 * k < p.dim / 8) to[c0 + 32 * k] = v[k];
+        }
       }
       if (p.dh != nullptr) {
         const int vecs = p.dim / (p.dh_f32 ? 4 : 8);
@@ -681,6 +718,137 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
     const int end = min(p.tokens, (all + kXK - 1) / kXK * kXK);
     for (int64_t c = (int64_t)all * (p.dim / 8) + threadIdx.x; c < (int64_t)end * (p.dim / 8); c += kPackThreads)
       reinterpret_cast<uint4*>(p.packed)[c] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// The forward statistics of one to four tokens: reading W is all there is to it, and whole rows in a row
+// read better than the tensor core's 128-byte columns of 256 rows (131072 x 4096, one token: FIGURES).  A warp
+// takes four neighbouring rows of W at a time, the tokens' states wait in shared memory as bf16; products
+// and sums in fp32.  One partial (maximum, sum) per block and token.
+constexpr int kRowsThreads = 256, kRowsPerWarp = 4, kRowsTokens = 4;
+constexpr int64_t kRowsElems = 24000;            // tokens * dim: 47 KB of shared memory
+struct RowsParams {
+  const __nv_bfloat16* h;
+  const __nv_bfloat16* w;
+  int64_t ldh, ldw;
+  const void* bias;
+  int bias_f32;
+  int dim, vocab, tokens;
+  const int* slots;
+  const int* token;
+  const int* target;
+  float2* part;                                  // [gridDim.x][tokens]
+  float* picked;
+};
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float acc) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    acc = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), acc);
+    acc = fmaf(__uint_as_float(x[i] & 0xFFFF0000u), __uint_as_float(y[i] & 0xFFFF0000u), acc);
+  }
+  return acc;
+}
+// adds one logit to a running (maximum, sum of exponentials)
+__device__ __forceinline__ void running_add(float x, float& m, float& s) {
+  const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.f : mn;
+  s = s * exp2_fast((m - ref) * kLog2e) + exp2_fast((x - ref) * kLog2e);
+  m = mn;
+}
+template <int kT>
+__global__ void __launch_bounds__(kRowsThreads) xent_rows_kernel(const RowsParams p) {
+  extern __shared__ __align__(16) uint4 state[];             // [kT][dim / 8]
+  __shared__ float2 red[kRowsThreads / 32][kT];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int slots = *static_cast<const volatile int*>(p.slots);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int vecs = p.dim / 8;
+  int target[kT];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) target[t] = t < slots ? p.target[t] : -1;
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+    const uint4* from = t < slots ? reinterpret_cast<const uint4*>(p.h + (int64_t)p.token[t] * p.ldh) : nullptr;
+    for (int c = threadIdx.x; c < vecs; c += kRowsThreads) state[t * vecs + c] = from ? from[c] : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __syncthreads();
+  float m[kT], s[kT];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+    m[t] = -INFINITY;
+    s[t] = 0.f;
+  }
+  const int stride = gridDim.x * (kRowsThreads / 32) * kRowsPerWarp;
+  for (int v0 = (blockIdx.x * (kRowsThreads / 32) + warp) * kRowsPerWarp; v0 < p.vocab && slots > 0; v0 += stride) {
+    const uint4* row[kRowsPerWarp];
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; ++r) row[r] = reinterpret_cast<const uint4*>(p.w + (int64_t)min(v0 + r, p.vocab - 1) * p.ldw);
+    float acc[kRowsPerWarp][kT];
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; ++r)
+#pragma unroll
+      for (int t = 0; t < kT; ++t) acc[r][t] = 0.f;
+    int c = lane;
+    for (; c + 96 < vecs; c += 128) {                        // sixteen 16-byte loads in flight per lane
+      uint4 q[4][kRowsPerWarp];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int r = 0; r < kRowsPerWarp; ++r) q[k][r] = __ldcs(row[r] + c + 32 * k);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          const uint4 hv = state[t * vecs + c + 32 * k];
+#pragma unroll
+          for (int r = 0; r < kRowsPerWarp; ++r) acc[r][t] = dot8(q[k][r], hv, acc[r][t]);
+        }
+    }
+    for (; c < vecs; c += 32) {
+      uint4 q[kRowsPerWarp];
+#pragma unroll
+      for (int r = 0; r < kRowsPerWarp; ++r) q[r] = __ldcs(row[r] + c);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const uint4 hv = state[t * vecs + c];
+#pragma unroll
+        for (int r = 0; r < kRowsPerWarp; ++r) acc[r][t] = dot8(q[r], hv, acc[r][t]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; ++r) {
+      const int v = v0 + r;
+      float b = 0.f;
+      if (p.bias != nullptr && v < p.vocab)
+        b = p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + v) : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[v]);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        float x = acc[r][t];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+        x += b;
+        if (v < p.vocab) {
+          running_add(x, m[t], s[t]);
+          if (lane == 0 && v == target[t]) p.picked[t] = x;
+        }
+      }
+    }
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) red[warp][t] = make_float2(m[t], s[t]);
+  }
+  __syncthreads();
+  if (threadIdx.x < kT && (int)threadIdx.x < p.tokens) {
+    float mm = -INFINITY, ss = 0.f;
+    for (int w = 0; w < kRowsThreads / 32; ++w) {
+      const float2 q = red[w][threadIdx.x];
+      const float mn = fmaxf(mm, q.x), ref = mn == -INFINITY ? 0.f : mn;
+      ss = ss * exp2_fast((mm - ref) * kLog2e) + q.y * exp2_fast((q.x - ref) * kLog2e);
+      mm = mn;
+    }
+    p.part[(int64_t)blockIdx.x * p.tokens + threadIdx.x] = make_float2(mm, ss);
   }
 }
 
@@ -780,23 +948,29 @@ struct SliceParams {
   const float* acc;
   void* out;
   int out_f32, rows, cols4, tokens;
-  const int* slots;
+  const int* slots;                      // dh: the splits are kProduct's own
   const int* token;
+  int n_tiles, k_stages, split_clusters;
 };
 __global__ void __launch_bounds__(256) xent_slices_kernel(const SliceParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  int rows = p.rows;
+  int rows = p.rows, n = p.n;
+  int64_t slice_elems = p.slice_elems;
   bool scatter = false;
   if (p.slots != nullptr) {
     rows = min(rows, *static_cast<const volatile int*>(p.slots));
     scatter = p.token != nullptr && rows < p.tokens;
+    const int m_tiles = (rows + kXM - 1) / kXM;
+    n = split_slots(m_tiles, p.n_tiles, p.k_stages, p.split_clusters).splits;
+    if (n == 1) return;                  // written by kProduct itself
+    slice_elems = (int64_t)m_tiles * kXM * p.cols4 * 4;
   }
   const int64_t total4 = (int64_t)rows * p.cols4;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total4; i += (int64_t)gridDim.x * 256) {
     float4 v = p.acc ? reinterpret_cast<const float4*>(p.acc)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.n; ++s) {
-      const float4 f = reinterpret_cast<const float4*>(p.slices + s * p.slice_elems)[i];
+    for (int s = 0; s < n; ++s) {
+      const float4 f = reinterpret_cast<const float4*>(p.slices + s * slice_elems)[i];
       v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
     }
     int64_t to = i;
@@ -814,10 +988,10 @@ __global__ void __launch_bounds__(256) xent_slices_kernel(const SliceParams p) {
 }
 
 // db: the column sums of dl that the gradient epilogue left per 32 slots (taken in fp32, before dl is
-// rounded).  A block per 32 columns; its 32 warps take the rows in turn and are added in warp order.
-__global__ void __launch_bounds__(1024) xent_bias_grad_kernel(const float* __restrict__ part, int64_t ld, const int* slots, int cols, void* db,
+// rounded).  A block per 32 columns; its 8 warps take the rows in turn and are added in warp order.
+__global__ void __launch_bounds__(256) xent_bias_grad_kernel(const float* __restrict__ part, int64_t ld, const int* slots, int cols, void* db,
                                                               int db_f32) {
-  __shared__ float red[32][32];
+  __shared__ float red[8][32];
   pdl_launch_dependents();
   pdl_wait();
   const int rows = (*static_cast<const volatile int*>(slots) + 31) / 32;
@@ -826,13 +1000,13 @@ __global__ void __launch_bounds__(1024) xent_bias_grad_kernel(const float* __res
   float a = 0.f;
   if (c < cols) {
 #pragma unroll 8
-    for (int r = warp; r < rows; r += 32) a += part[(int64_t)r * ld + c];
+    for (int r = warp; r < rows; r += 8) a += part[(int64_t)r * ld + c];
   }
   red[warp][lane] = a;
   __syncthreads();
   if (warp == 0 && c < cols) {
     float s = 0.f;
-    for (int w = 0; w < 32; ++w) s += red[w][lane];
+    for (int w = 0; w < 8; ++w) s += red[w][lane];
     if (db_f32) static_cast<float*>(db)[c] = s;
     else static_cast<__nv_bfloat16*>(db)[c] = __float2bfloat16_rn(s);
   }
@@ -874,19 +1048,23 @@ int cluster_budget() {
   return sms > 0 ? std::max(1, sms / 2) : -1;
 }
 
+int64_t round_up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
+
+int width_for(int64_t cols) { return cols <= 128 ? 128 : 256; }     // of a tile
+
 // How a product [m, n] over k is cut: tile width, and K splits when its tiles leave most clusters idle.
 struct Cut {
   int bn = 256, splits = 1, ks_per_split = 0;
   int64_t slice_rows = 0;
   int64_t slice_bytes(int64_t n) const { return splits > 1 ? splits * slice_rows * n * 4 : 0; }
 };
-Cut cut_product(int64_t m, int64_t n, int64_t k, bool may_split, int clusters) {
+Cut cut_product(int64_t m, int64_t n, int64_t k, int clusters) {
   Cut c;
   const int64_t mt = ceil_div(m, kXM), stages = ceil_div(k, kXK);
-  c.bn = n <= 128 ? 128 : 256;
+  c.bn = width_for(n);
   const int64_t tiles = mt * ceil_div(n, c.bn);
   c.ks_per_split = (int)stages;
-  if (may_split && tiles * 2 <= clusters && stages >= 4) {
+  if (tiles * 2 <= clusters && stages >= 4) {
     int64_t s = std::min<int64_t>(clusters / tiles, stages / 2);
     if (s >= 2) {
       c.ks_per_split = (int)ceil_div(stages, s);
@@ -906,7 +1084,8 @@ int bf16_map(CUtensorMap* map, const Operand& o, int box_inner, int box_outer, C
                               (uint32_t)box_inner, (uint32_t)box_outer, sw);
 }
 
-// `packed`: the counted tokens' rows of h, read in place of operand a (kStats, kGrad) or b (kProductT)
+// `packed`: the counted tokens' rows of h, read in place of operand a (kStats, kGrad) or b (kProductT); for
+// kProduct the fp32 slices.
 template <int kMode, int kBN>
 int launch_width(const Operand& a, const Operand& b, const Operand& packed, void* out, int64_t ldo, XParams g, int64_t k, cudaStream_t stream) {
   using C = XCfg<kBN>;
@@ -931,6 +1110,9 @@ int launch_width(const Operand& a, const Operand& b, const Operand& packed, void
   int rc = kAMn ? bf16_map(&map_a, a, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_a, a, kXK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == FP4T_OK)
     rc = kBMn ? bf16_map(&map_b, b, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_b, b, kXK, C::kBRows, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == FP4T_OK && kMode == kProduct && g.split_clusters > 0)
+    rc = encode_tensor_map_2d(&map_packed, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, packed.p, (uint64_t)packed.inner, (uint64_t)packed.outer,
+                              (uint64_t)packed.ld * 4, 32u, 32u, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == FP4T_OK && kMode != kProduct)
     rc = kBMn ? bf16_map(&map_packed, packed, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_packed, packed, kXK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == FP4T_OK && kMode != kStats) {
@@ -939,7 +1121,7 @@ int launch_width(const Operand& a, const Operand& b, const Operand& packed, void
                               (uint64_t)ldo * (g.out_f32 ? 4 : 2), 32u, 32u, g.out_f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   }
   if (rc != FP4T_OK) return rc;
-  const int64_t units = (int64_t)g.m_tiles * g.n_tiles * g.splits;
+  const int64_t units = kMode == kProduct && g.split_clusters > 0 ? clusters : (int64_t)g.m_tiles * g.n_tiles * g.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(units, clusters)), 1, 1);
   cfg.blockDim = dim3(kXThreads, 1, 1);
@@ -962,10 +1144,11 @@ int launch_xent(int bn, const Operand& a, const Operand& b, const Operand& packe
 }
 
 template <typename... Args, typename... Actual>
-int launch_small(void (*kern)(Args...), int grid, int threads, cudaStream_t stream, Actual... args) {
+int launch_small_shared(void (*kern)(Args...), int grid, int threads, int64_t shared, cudaStream_t stream, Actual... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)shared;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   pdl_attribute(&attr);
@@ -973,6 +1156,10 @@ int launch_small(void (*kern)(Args...), int grid, int threads, cudaStream_t stre
   cfg.numAttrs = 1;
   FP4T_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
   return FP4T_OK;
+}
+template <typename... Args, typename... Actual>
+int launch_small(void (*kern)(Args...), int grid, int threads, cudaStream_t stream, Actual... args) {
+  return launch_small_shared(kern, grid, threads, 0, stream, args...);
 }
 
 // What both passes know about the counted tokens (device memory in the workspace).
@@ -984,50 +1171,66 @@ struct Slots {
   __nv_bfloat16* packed;
 };
 
-// One product into `out` (contiguous rows of `cols`), through slices when it is split.  to_tokens: its rows
-// are slots in the product and tokens in `out`.
-template <int kMode>
-int run_product(const Cut& cut, const Operand& a, const Operand& b, const Operand& packed, int64_t k, int64_t rows, int64_t cols, int64_t tokens,
-                void* out, int out_f32, bool to_tokens, const float* acc, float* slices, const Slots& sl, int32_t* status, cudaStream_t stream) {
+// dh (or its sum over the pieces so far) into `out`, rows of `dim`: slots, or tokens' places if to_tokens.
+int run_dh(const Operand& dl, const Operand& w, int64_t tokens, int64_t dim, int64_t vc, void* out, int out_f32, bool to_tokens, const float* acc,
+           float* slices, int64_t slice_rows, int split_clusters, const Slots& sl, int32_t* status, cudaStream_t stream) {
   XParams g = {};
-  g.rows = (int)rows;
-  g.cols = (int)cols;
-  g.tokens = (int)tokens;
+  g.rows = g.tokens = (int)tokens;
+  g.cols = (int)dim;
   g.slots = sl.slots;
   g.token = sl.token;
   g.status = status;
   g.out_f32 = out_f32;
-  g.splits = cut.splits;
-  g.ks_per_split = cut.ks_per_split;
-  if (cut.splits == 1) {
-    g.acc = acc;
-    g.ldacc = cols;
-    g.out = to_tokens ? out : nullptr;
-    return launch_xent<kMode>(cut.bn, a, b, packed, out, cols, g, k, stream);
-  }
-  g.slice_rows = (int)cut.slice_rows;
-  g.out_f32 = 1;
-  int rc = launch_xent<kMode>(cut.bn, a, b, packed, slices, cols, g, k, stream);
-  if (rc != FP4T_OK) return rc;
+  g.acc = acc;
+  g.ldacc = dim;
+  g.out = to_tokens ? out : nullptr;
+  const int bn = width_for(dim);
+  split_clusters = std::min(split_clusters, bn == 128 ? xent_clusters<kProduct, 128>() : xent_clusters<kProduct, 256>());
+  g.split_clusters = slice_rows > 0 ? split_clusters : 0;      // (the kernel's launch refuses when none can be resident)
+  int rc = launch_xent<kProduct>(bn, dl, w, Operand{slices, slice_rows, dim, dim}, out, dim, g, vc, stream);
+  if (rc != FP4T_OK || g.split_clusters <= 0) return rc;
   SliceParams p = {};
   p.slices = slices;
-  p.n = cut.splits;
-  p.slice_elems = cut.slice_rows * cols;
   p.acc = acc;
   p.out = out;
   p.out_f32 = out_f32;
-  p.rows = (int)rows;
-  p.cols4 = (int)(cols / 4);
-  p.tokens = (int)tokens;
-  p.slots = kMode == kProduct ? sl.slots : nullptr;
+  p.rows = p.tokens = (int)tokens;
+  p.cols4 = (int)(dim / 4);
+  p.slots = sl.slots;
   p.token = to_tokens ? sl.token : nullptr;
-  const int grid = (int)std::min<int64_t>(ceil_div(rows * cols / 4, 256), 148 * 8);
+  p.n_tiles = (int)ceil_div(dim, bn);
+  p.k_stages = (int)ceil_div(vc, kXK);
+  p.split_clusters = split_clusters;
+  const int grid = (int)std::min<int64_t>(ceil_div(std::min(tokens, slice_rows) * dim / 4, 256), 148 * 8);
   return launch_small(xent_slices_kernel, grid, 256, stream, p);
 }
 
-int64_t round_up(int64_t v, int64_t to) { return ceil_div(v, to) * to; }
-
-int width_for(int64_t vocab) { return vocab <= 128 ? 128 : 256; }   // of a tile of logits
+// dW's rows of a piece, through slices when it is split (few entries, many tokens).
+int run_dw(const Cut& cut, const Operand& dl, const Operand& h, const Operand& packed, int64_t tokens, int64_t dim, int64_t vc, void* out, int out_f32,
+           float* slices, const Slots& sl, int32_t* status, cudaStream_t stream) {
+  XParams g = {};
+  g.rows = (int)vc;
+  g.cols = (int)dim;
+  g.tokens = (int)tokens;
+  g.slots = sl.slots;
+  g.status = status;
+  g.splits = cut.splits;
+  g.ks_per_split = cut.ks_per_split;
+  g.out_f32 = cut.splits > 1 ? 1 : out_f32;
+  g.slice_rows = (int)cut.slice_rows;
+  int rc = launch_xent<kProductT>(cut.bn, dl, h, packed, cut.splits > 1 ? slices : out, dim, g, tokens, stream);
+  if (rc != FP4T_OK || cut.splits == 1) return rc;
+  SliceParams p = {};
+  p.slices = slices;
+  p.n = cut.splits;
+  p.slice_elems = cut.slice_rows * dim;
+  p.out = out;
+  p.out_f32 = out_f32;
+  p.rows = (int)vc;
+  p.cols4 = (int)(dim / 4);
+  const int grid = (int)std::min<int64_t>(ceil_div(vc * dim / 4, 256), 148 * 8);
+  return launch_small(xent_slices_kernel, grid, 256, stream, p);
+}
 
 // Slots in the workspace: their number, the token and target of each, counts per run, the packed rows of h.
 struct SlotPlan {
@@ -1035,7 +1238,7 @@ struct SlotPlan {
 };
 SlotPlan plan_slots(int64_t tokens, int64_t dim) {
   SlotPlan p;
-  p.run = std::max<int64_t>(32, round_up(ceil_div(tokens, 148 * 4), 32));
+  p.run = round_up(ceil_div(tokens, 148 * 4), 8);        // a warp copies a row at a time, a block has eight
   p.runs = ceil_div(tokens, p.run);
   p.o_token = 256;                       // slot count at 0, joining kernel's counter at 128
   p.o_target = p.o_token + round_up(tokens * 4, 128);
@@ -1079,6 +1282,7 @@ int launch_pack(const SlotPlan& plan, const Slots& sl, const void* h, int64_t ld
 // Forward workspace: slots, the joining blocks' sums, the targets' logits, partial statistics of a block of slots.
 struct ForwardPlan {
   SlotPlan slots;
+  int64_t rows_blocks;                    // blocks of the few-tokens kernel, 0: the tensor-core one
   int64_t block, parts, join_blocks;      // slots per block, partials per slot, joining blocks of all blocks of slots
   int lanes;
   int64_t o_loss, o_picked, o_part, bytes;
@@ -1087,7 +1291,8 @@ ForwardPlan plan_forward(int64_t tokens, int64_t dim, int64_t vocab) {
   ForwardPlan p;
   p.slots = plan_slots(tokens, dim);
   p.block = std::min(tokens, kTokenBlock);
-  p.parts = 2 * ceil_div(vocab, width_for(vocab));
+  p.rows_blocks = tokens <= kRowsTokens && (tokens == 3 ? 4 : tokens) * dim <= kRowsElems ? std::min<int64_t>(ceil_div(vocab, kRowsThreads / 32 * kRowsPerWarp), 148 * 2) : 0;
+  p.parts = p.rows_blocks > 0 ? p.rows_blocks : 2 * ceil_div(vocab, width_for(vocab));
   p.lanes = 1;
   while (p.lanes < 8 && p.lanes < tokens) p.lanes <<= 1;
   p.join_blocks = (tokens / p.block) * ceil_div(p.block, p.lanes) + ceil_div(tokens % p.block, p.lanes);
@@ -1102,7 +1307,8 @@ ForwardPlan plan_forward(int64_t tokens, int64_t dim, int64_t vocab) {
 struct BackwardPlan {
   SlotPlan slots;
   int64_t piece, pieces, ld;
-  Cut dh, dw;
+  Cut dw;
+  int64_t dh_slice_rows;                    // of dh's slices, all splits together; 0: never split
   int64_t o_dl, o_acc, o_cols, o_slices, bytes;
 };
 BackwardPlan plan_backward(int64_t tokens, int64_t dim, int64_t vocab, bool want_dh, bool want_dw, bool want_db, int clusters) {
@@ -1113,13 +1319,14 @@ BackwardPlan plan_backward(int64_t tokens, int64_t dim, int64_t vocab, bool want
   p.piece = round_up(ceil_div(vocab, p.pieces), 256);       // even pieces
   p.pieces = ceil_div(vocab, p.piece);
   p.ld = std::min(p.piece, round_up(vocab, 8));
-  p.dh = cut_product(tokens, dim, std::min(p.piece, vocab), true, clusters);
-  p.dw = cut_product(std::min(p.piece, vocab), dim, tokens, true, clusters);
+  p.dw = cut_product(std::min(p.piece, vocab), dim, tokens, clusters);
+  const int64_t dh_tiles = ceil_div(dim, width_for(dim));
+  p.dh_slice_rows = want_dh && dh_tiles * 2 <= clusters && ceil_div(std::min(p.piece, vocab), kXK) >= 4 ? clusters / dh_tiles * kXM : 0;
   p.o_dl = p.slots.bytes;
   p.o_acc = p.o_dl + round_up(tokens * p.ld * 2, 1024);
   p.o_cols = p.o_acc + (want_dh && p.pieces > 1 ? round_up(tokens * dim * 4, 1024) : 0);
   p.o_slices = p.o_cols + (want_db ? round_up(round_up(tokens, kXK) / 32 * p.ld * 4, 1024) : 0);
-  p.bytes = p.o_slices + std::max(want_dh ? p.dh.slice_bytes(dim) : 0, want_dw ? p.dw.slice_bytes(dim) : 0);
+  p.bytes = p.o_slices + std::max(p.dh_slice_rows * dim * 4, want_dw ? p.dw.slice_bytes(dim) : 0);
   return p;
 }
 
@@ -1192,7 +1399,26 @@ extern "C" int fp4t_linear_xent_forward(const void* h, int64_t ldh, const void* 
     g.part = reinterpret_cast<float2*>(ws + p.o_part);
     g.picked = reinterpret_cast<float*>(ws + p.o_picked);
     g.status = status;
-    rc = launch_xent<kStats>(width_for(vocab), Operand{static_cast<const __nv_bfloat16*>(h) + t0 * ldh, rows, dim, ldh}, Operand{w, vocab, dim, ldw},
+    if (p.rows_blocks > 0) {
+      RowsParams r = {};
+      r.h = static_cast<const __nv_bfloat16*>(h);
+      r.w = static_cast<const __nv_bfloat16*>(w);
+      r.ldh = ldh;
+      r.ldw = ldw;
+      r.bias = bias;
+      r.bias_f32 = g.bias_f32;
+      r.dim = (int)dim;
+      r.vocab = (int)vocab;
+      r.tokens = (int)tokens;
+      r.slots = sl.slots;
+      r.token = sl.token;
+      r.target = sl.target;
+      r.part = g.part;
+      r.picked = g.picked;
+      auto kern = tokens == 1 ? xent_rows_kernel<1> : tokens == 2 ? xent_rows_kernel<2> : xent_rows_kernel<4>;
+      rc = launch_small_shared(kern, (int)p.rows_blocks, kRowsThreads, (tokens <= 2 ? tokens : 4) * dim * 2, s, r);
+    } else
+      rc = launch_xent<kStats>(width_for(vocab), Operand{static_cast<const __nv_bfloat16*>(h) + t0 * ldh, rows, dim, ldh}, Operand{w, vocab, dim, ldw},
                              Operand{sl.packed + t0 * dim, rows, dim, dim}, nullptr, 0, g, dim, s);
     if (rc != FP4T_OK) return rc;
     JoinParams j = {};
@@ -1287,24 +1513,18 @@ extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, 
     if (rc != FP4T_OK) return rc;
     if (dh) {
       const bool last = i == p.pieces - 1;
-      Cut cut = p.dh;
-      if (vc != std::min(p.piece, vocab)) {            // a shorter last piece: the same slices, fewer of them
-        const int64_t stages = ceil_div(vc, kXK);
-        cut.ks_per_split = (int)std::min<int64_t>(cut.ks_per_split, stages);
-        cut.splits = (int)std::min<int64_t>(cut.splits, ceil_div(stages, cut.ks_per_split));
-      }
-      rc = run_product<kProduct>(cut, dop, wop, packed, vc, tokens, dim, tokens, last ? dh : static_cast<void*>(acc),
-                                 last ? dh_dtype == FP4T_DT_F32 : 1, last, i > 0 ? acc : nullptr, slices, sl, status, s);
+      rc = run_dh(dop, wop, tokens, dim, vc, last ? dh : static_cast<void*>(acc), last ? dh_dtype == FP4T_DT_F32 : 1, last, i > 0 ? acc : nullptr,
+                  slices, p.dh_slice_rows, clusters, sl, status, s);
       if (rc != FP4T_OK) return rc;
     }
     if (dw) {
       void* out = static_cast<uint8_t*>(dw) + v0 * dim * (dw_dtype == FP4T_DT_F32 ? 4 : 2);
-      rc = run_product<kProductT>(p.dw, dop, hop, packed, tokens, vc, dim, tokens, out, dw_dtype == FP4T_DT_F32, false, nullptr, slices, sl, status, s);
+      rc = run_dw(p.dw, dop, hop, packed, tokens, dim, vc, out, dw_dtype == FP4T_DT_F32, slices, sl, status, s);
       if (rc != FP4T_OK) return rc;
     }
     if (db) {
       void* out = static_cast<uint8_t*>(db) + v0 * (db_dtype == FP4T_DT_F32 ? 4 : 2);
-      rc = launch_small(xent_bias_grad_kernel, (int)ceil_div(vc, 32), 1024, s, (const float*)g.col_part, p.ld, (const int*)sl.slots, (int)vc, out,
+      rc = launch_small(xent_bias_grad_kernel, (int)ceil_div(vc, 32), 256, s, (const float*)g.col_part, p.ld, (const int*)sl.slots, (int)vc, out,
                         (int)(db_dtype == FP4T_DT_F32));
       if (rc != FP4T_OK) return rc;
     }

@@ -724,97 +724,118 @@ def qk_norm_rotary_backward(dy, x, weights, eps, positions=None, table=None):
 
 # ------------------------------------------------------------------ linear cross entropy
 def _xent_rows(t, name):
-    """2-D bf16 tensor with rows the kernels can load: unit column stride, 16-byte aligned rows."""
-    _need_cuda(t)
-    if t.ndim != 2 or t.dtype != torch.bfloat16:
+    """2-D bf16 tensor with rows the kernels can load (unit column stride, 16-byte aligned rows); its pitch."""
+    if not t.is_cuda:
+        _need_cuda(t)
+    if t.ndim != 2 or t.dtype is not torch.bfloat16:
         raise ValueError(f"linear_cross_entropy: {name} must be a 2-D bfloat16 tensor")
     rows, dim = t.shape
-    if t.stride(1) != 1 or t.data_ptr() % 16 or (rows > 1 and (t.stride(0) % 8 or t.stride(0) < dim)):
+    ld, unit = t.stride()
+    if rows <= 1:
+        ld = dim
+    if unit != 1 or ld % 8 or ld < dim or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t, (t.stride(0) if rows > 1 else dim)
+        ld = dim
+    return t, ld
 
 
 def _xent_args(h, w, bias, target, reduction):
     h, ldh = _xent_rows(h, "hidden")
     w, ldw = _xent_rows(w, "weight")
-    _need_cuda(target, bias)
-    if h.shape[1] != w.shape[1]:
-        raise ValueError(f"linear_cross_entropy: hidden is {h.shape[1]} wide, weight {w.shape[1]}")
-    if h.shape[1] % 8 or h.shape[1] == 0:
-        raise ValueError(f"linear_cross_entropy needs a width that is a multiple of 8, got {h.shape[1]}")
-    if w.shape[0] == 0:
+    T, D = h.shape
+    V, dim = w.shape
+    if not target.is_cuda:
+        _need_cuda(target)
+    if dim != D:
+        raise ValueError(f"linear_cross_entropy: hidden is {D} wide, weight {dim}")
+    if D % 8 or D == 0:
+        raise ValueError(f"linear_cross_entropy needs a width that is a multiple of 8, got {D}")
+    if V == 0:
         raise ValueError("linear_cross_entropy: the vocabulary is empty")
-    if target.shape != (h.shape[0],) or target.dtype != torch.int64:
-        raise ValueError(f"linear_cross_entropy: target must be int64 [{h.shape[0]}]")
+    if target.ndim != 1 or target.shape[0] != T or target.dtype is not torch.int64:
+        raise ValueError(f"linear_cross_entropy: target must be int64 [{T}]")
     if reduction not in _lib.XENT_REDUCTION:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    dev = h.device
     if bias is not None:
-        if bias.shape != (w.shape[0],) or bias.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"linear_cross_entropy: bias must be float32 or bfloat16 [{w.shape[0]}]")
-        bias = bias.contiguous()
-        if bias.data_ptr() % 16:
-            bias = bias.clone()
-    for t in (w, target, bias):
-        if t is not None and t.device != h.device:
-            raise ValueError("linear_cross_entropy: all tensors must be on one device")
-    return h, ldh, w, ldw, bias, target.contiguous()
+        _need_cuda(bias)
+        if bias.ndim != 1 or bias.shape[0] != V or bias.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"linear_cross_entropy: bias must be float32 or bfloat16 [{V}]")
+        if not bias.is_contiguous() or bias.data_ptr() % 16:
+            bias = bias.contiguous()
+            bias = bias if bias.data_ptr() % 16 == 0 else bias.clone()
+    if w.device != dev or target.device != dev or (bias is not None and bias.device != dev):
+        raise ValueError("linear_cross_entropy: all tensors must be on one device")
+    if not target.is_contiguous():
+        target = target.contiguous()
+    return h, ldh, w, ldw, bias, target, T, D, V
+
+
+def _code(dtype):
+    return int(dtype is torch.float32)      # FP4T_DT_BF16 = 0, FP4T_DT_F32 = 1
 
 
 def linear_cross_entropy_forward(h, w, bias, target, ignore_index=-100, reduction="mean"):
     """Cross entropy of h @ w.T + bias without the logits.  h [T, D], w [V, D] bf16, bias [V] fp32 / bf16 or
     None, target [T] int64 -> (loss [] or, reduction "none", [T]; lse [T],
     of the counted tokens in order; count []), all fp32."""
-    h, ldh, w, ldw, bias, target = _xent_args(h, w, bias, target, reduction)
-    dev, (T, D), V = h.device, h.shape, w.shape[0]
-    with _on_device(dev):
+    h, ldh, w, ldw, bias, target, T, D, V = _xent_args(h, w, bias, target, reduction)
+    index, dev = h.get_device(), h.device
+    with _device_context(index):
         stats = torch.empty(T + 1, dtype=torch.float32, device=dev)
         lse, count = stats[:T], stats[T]
         if T == 0:
             count.zero_()
-            empty = {"none": 0, "sum": 1, "mean": 1}[reduction]
-            return torch.full((empty,) if not empty else (), float("nan") if reduction == "mean" else 0.0, device=dev), lse, count
+            shape = (0,) if reduction == "none" else ()
+            return torch.full(shape, float("nan") if reduction == "mean" else 0.0, device=dev), lse, count
         loss = torch.empty(T if reduction == "none" else (), dtype=torch.float32, device=dev)
         L = _lib.lib()
         ws_bytes = L.fp4t_linear_xent_forward_workspace_bytes(T, D, V)
         if ws_bytes < 0:
             _lib.check(-1, "fp4t_linear_xent_forward_workspace_bytes")
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        rc = L.fp4t_linear_xent_forward(h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias),
-                                        0 if bias is None else _lib.dtype_code(bias.dtype), target.data_ptr(), T, D, V,
-                                        int(ignore_index), _lib.XENT_REDUCTION[reduction], loss.data_ptr(), lse.data_ptr(),
-                                        count.data_ptr(), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+        at = stats.data_ptr()
+        rc = L.fp4t_linear_xent_forward(h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias), 0 if bias is None else _code(bias.dtype),
+                                        target.data_ptr(), T, D, V, ignore_index, _lib.XENT_REDUCTION[reduction], loss.data_ptr(), at,
+                                        at + 4 * T, ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(),
+                                        torch._C._cuda_getCurrentRawStream(index))
+    if rc:
         _lib.check(rc, "fp4t_linear_xent_forward")
-        LAUNCHES["xent"] += 1 + 2 * (-(-T // 16384))
+    LAUNCHES["xent"] += 1 + 2 * (-(-T // 16384))
     return loss, lse, count
 
 
 def linear_cross_entropy_backward(grad_loss, h, w, bias, target, lse, ignore_index=-100, reduction="mean",
                                   dh_dtype=None, dw_dtype=None, db_dtype=None):
     """-> (dh [T, D], dw [V, D], db [V]) in the dtypes asked for (None: not computed) for the forward above."""
-    h, ldh, w, ldw, bias, target = _xent_args(h, w, bias, target, reduction)
-    dev, (T, D), V = h.device, h.shape, w.shape[0]
-    _need_cuda(grad_loss, lse)
-    grad_loss = grad_loss.to(torch.float32).contiguous()
-    if grad_loss.numel() != (T if reduction == "none" else 1):
-        raise ValueError("linear_cross_entropy: grad_loss must have the shape of the loss")
-    with _on_device(dev):
-        make = lambda shape, dt: None if dt is None else (torch.zeros if T == 0 else torch.empty)(shape, dtype=dt, device=dev)  # noqa: E731
-        dh, dw, db = make((T, D), dh_dtype), make((V, D), dw_dtype), make((V,), db_dtype)
+    h, ldh, w, ldw, bias, target, T, D, V = _xent_args(h, w, bias, target, reduction)
+    if not (grad_loss.is_cuda and lse.is_cuda):
+        _need_cuda(grad_loss, lse)
+    if grad_loss.dtype is not torch.float32 or not grad_loss.is_contiguous():
+        grad_loss = grad_loss.to(torch.float32).contiguous()
+    if grad_loss.numel() != (T if reduction == "none" else 1) or lse.numel() != T or lse.dtype is not torch.float32 or not lse.is_contiguous():
+        raise ValueError("linear_cross_entropy: grad_loss must have the shape of the loss, lse that of the forward's")
+    index, dev = h.get_device(), h.device
+    with _device_context(index):
+        make = torch.empty if T else torch.zeros
+        dh = None if dh_dtype is None else make((T, D), dtype=dh_dtype, device=dev)
+        dw = None if dw_dtype is None else make((V, D), dtype=dw_dtype, device=dev)
+        db = None if db_dtype is None else make((V,), dtype=db_dtype, device=dev)
         if T == 0 or (dh is None and dw is None and db is None):
             return dh, dw, db
         L = _lib.lib()
-        ws_bytes = L.fp4t_linear_xent_backward_workspace_bytes(T, D, V, int(dh is not None), int(dw is not None), int(db is not None))
+        ws_bytes = L.fp4t_linear_xent_backward_workspace_bytes(T, D, V, dh is not None, dw is not None, db is not None)
         if ws_bytes < 0:
             raise RuntimeError("fp4t_linear_xent_backward_workspace_bytes: unsupported shape or device")
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        code = lambda t: 0 if t is None else _lib.dtype_code(t.dtype)  # noqa: E731
-        rc = L.fp4t_linear_xent_backward(grad_loss.data_ptr(), h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias), code(bias),
-                                         target.data_ptr(), lse.data_ptr(), T, D, V, int(ignore_index),
-                                         _lib.XENT_REDUCTION[reduction], _lib.ptr(dh), code(dh), _lib.ptr(dw), code(dw),
-                                         _lib.ptr(db), code(db), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(),
-                                         _lib.stream_ptr(dev))
+        rc = L.fp4t_linear_xent_backward(grad_loss.data_ptr(), h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias),
+                                         0 if bias is None else _code(bias.dtype), target.data_ptr(), lse.data_ptr(), T, D, V, ignore_index,
+                                         _lib.XENT_REDUCTION[reduction], _lib.ptr(dh), _code(dh_dtype), _lib.ptr(dw), _code(dw_dtype),
+                                         _lib.ptr(db), _code(db_dtype), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(),
+                                         torch._C._cuda_getCurrentRawStream(index))
+    if rc:
         _lib.check(rc, "fp4t_linear_xent_backward")
-        LAUNCHES["xent"] += 2 + int(dh is not None) + int(dw is not None) + int(db is not None)
+    LAUNCHES["xent"] += 2 + (dh is not None) + (dw is not None) + (db is not None)
     return dh, dw, db

@@ -15,8 +15,7 @@
 // HBM-bound (forward 4 bytes per bf16 element, norm backward 6).  A group walks heads of ONE token,
 // queries and keys, with the cosines and sines of its pairs in registers: no shared memory, no barrier, and
 // the trigonometry is paid once per token, not per head.  Several heads' vectors are loaded before the
-// first is worked on, the first ones before the angles are computed.  Where tokens are few, a token's
-// heads are dealt out to several groups.
+// first is worked on, the first ones before the angles are computed.
 #include <algorithm>
 
 #include "fp4t_common.cuh"
@@ -24,10 +23,10 @@
 namespace fp4t {
 namespace {
 
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
 constexpr int kRotWarps = kRotThreads / 32;
 constexpr int kRotMaxDim = 512;           // 256 pairs: 32 lanes x 8
-constexpr int kRotBlocksPerSm = 2;        // of the norm backward: resident at once, and rows of its workspace
+constexpr int kRotBlocksPerSm = 4;        // of the norm backward: resident at once, and rows of its workspace
 
 struct HeadsIn {
   const void* p;
@@ -121,13 +120,21 @@ __device__ __forceinline__ void store_vec(T* p, const float* v) {
 
 // Cosine and sine of a fraction of a turn held in 64 bits (the integer part has wrapped away).  The
 // nearest quarter turn is taken off as an integer, so the float that is left is at most an eighth of
-// a turn and its rounding stays below 2^-25 of a quarter; the quarter swaps and negates.
+// a turn and its rounding stays below 2^-25 of a quarter; the quarter swaps and negates.  For bf16 tensors the
+// hardware's approximations serve: off by 2^-20 at most, 2^-11 of a bf16 step.
+template <bool kPrecise>
 __device__ __forceinline__ float2 turn_cos_sin(uint64_t fraction) {
   const uint32_t hi = (uint32_t)(fraction >> 32);
   const uint32_t quarter = (hi + 0x20000000u) >> 30;
   const int32_t rest = (int32_t)(hi - (quarter << 30));          // 2^-32 turns, |rest| <= 2^29
   float s, c;
-  sincospif((float)rest * 0x1p-31f, &s, &c);                     // half turns
+  if constexpr (kPrecise) {
+    sincospif((float)rest * 0x1p-31f, &s, &c);                   // half turns
+  } else {
+    const float x = (float)rest * 1.4629180792671596e-9f;        // 2 pi / 2^32
+    s = __sinf(x);
+    c = __cosf(x);
+  }
   const float a = (quarter & 1u) ? s : c, b = (quarter & 1u) ? c : s;
   return make_float2((quarter + 1u) & 2u ? -a : a, quarter & 2u ? -b : b);
 }
@@ -153,6 +160,48 @@ __device__ __forceinline__ void chunk_offsets(int p0, int turned, int& ea, int& 
 
 enum { kRotate = 0, kNormRotate = 1, kNormRotateBackward = 2 };
 
+// Two floats in one 64-bit register pair, worked on by one instruction (the norm kernels are bound by
+// instruction issue otherwise: 211 per lane and head without, see below); one float where chunks are single pairs.
+template <int W>
+struct Pack {
+  uint64_t v;
+  static __device__ __forceinline__ Pack of(const float* p) {
+    Pack r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(p[0]), "f"(p[1]));
+    return r;
+  }
+  static __device__ __forceinline__ Pack all(float x) {
+    const float t[2] = {x, x};
+    return of(t);
+  }
+  __device__ __forceinline__ void to(float* p) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(p[0]), "=f"(p[1]) : "l"(v)); }
+  __device__ __forceinline__ float sum() const {
+    float t[2];
+    to(t);
+    return t[0] + t[1];
+  }
+};
+template <>
+struct Pack<1> {
+  float v;
+  static __device__ __forceinline__ Pack of(const float* p) { return Pack{p[0]}; }
+  static __device__ __forceinline__ Pack all(float x) { return Pack{x}; }
+  __device__ __forceinline__ void to(float* p) const { p[0] = v; }
+  __device__ __forceinline__ float sum() const { return v; }
+};
+__device__ __forceinline__ Pack<2> mul(Pack<2> a, Pack<2> b) {
+  Pack<2> r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pack<2> fma(Pack<2> a, Pack<2> b, Pack<2> c) {
+  Pack<2> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pack<1> mul(Pack<1> a, Pack<1> b) { return Pack<1>{a.v * b.v}; }
+__device__ __forceinline__ Pack<1> fma(Pack<1> a, Pack<1> b, Pack<1> c) { return Pack<1>{fmaf(a.v, b.v, c.v)}; }
+
 // What a lane holds of a head: kSlots chunks of V pairs each (V * kSlots = 8 pairs), chunk s of lane j
 // starting at pair (j + s * group) * V.
 template <typename T, int V, bool kHalf>
@@ -167,47 +216,93 @@ struct LaneView {
       const int p0 = (lane + s * p.group) * V;
       has[s] = p0 < p.pairs;
       turns[s] = p0 < p.turned;
-      chunk_offsets<V, kHalf>(p0, p.turned, ea[s], eb[s]);
+      // a lane without a chunk loads the head's first one and is left out of sums and stores
+      chunk_offsets<V, kHalf>(has[s] ? p0 : 0, p.turned, ea[s], eb[s]);
     }
   }
   struct Head {
     Raw<T, V> a[kSlots], b[kSlots];
   };
-  __device__ __forceinline__ void load(const T* x, bool live, Head& r) const {
+  __device__ __forceinline__ void load(const T* x, Head& r) const {
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
-      if (live && has[s]) {
-        r.a[s].load(x + ea[s]);
-        r.b[s].load(x + eb[s]);
-      } else {
-        r.a[s].zero();
-        r.b[s].zero();
-      }
+      r.a[s].load(x + ea[s]);
+      r.b[s].load(x + eb[s]);
     }
   }
-  __device__ __forceinline__ void expand(const Head& r, float (&e)[16]) const {
+  // A lane's pairs as packs: first members in a, second ones in b; pack j belongs to chunk slot(j).
+  static constexpr int W = V == 1 ? 1 : 2, kPacks = 8 / W;
+  static __device__ __forceinline__ constexpr int slot(int j) { return j * W / V; }
+  using P = Pack<W>;
+  static __device__ __forceinline__ void pairs(const float (&e)[16], P (&a)[kPacks], P (&b)[kPacks]) {
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      const int at = 2 * V * slot(j), i = j * W % V;           // chunk, and pair in it
+      float t[2], u[2];
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        t[k] = e[at + (kHalf ? i + k : 2 * (i + k))];
+        u[k] = e[at + (kHalf ? V + i + k : 2 * (i + k) + 1)];
+      }
+      a[j] = P::of(t);
+      b[j] = P::of(u);
+    }
+  }
+  __device__ __forceinline__ void expand(const Head& r, P (&a)[kPacks], P (&b)[kPacks]) const {
+    float e[16];
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       r.a[s].expand(e + 2 * V * s);
       r.b[s].expand(e + 2 * V * s + V);
     }
+    pairs(e, a, b);
   }
-  __device__ __forceinline__ void load_weight(const float* w, float (&e)[16]) const {
+  __device__ __forceinline__ void load_weight(const float* w, P (&wa)[kPacks], P (&wb)[kPacks]) const {
+    float e[16];
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       Raw<float, V> a, b;
-      if (has[s]) {
-        a.load(w + ea[s]);
-        b.load(w + eb[s]);
-      } else {
-        a.zero();
-        b.zero();
-      }
+      a.load(w + ea[s]);
+      b.load(w + eb[s]);
       a.expand(e + 2 * V * s);
       b.expand(e + 2 * V * s + V);
     }
+    pairs(e, wa, wb);
   }
-  __device__ __forceinline__ void store(T* y, const float (&e)[16]) const {
+  // sum of a b + c d over what the lane holds
+  __device__ __forceinline__ float sum_of_products(const P (&a)[kPacks], const P (&b)[kPacks], const P (&c)[kPacks], const P (&d)[kPacks]) const {
+    float total = 0.f;
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      constexpr int kPer = V / W;                              // packs of a chunk
+      P x = mul(a[s * kPer], b[s * kPer]), y = mul(c[s * kPer], d[s * kPer]);
+#pragma unroll
+      for (int j = 1; j < kPer; ++j) {
+        x = fma(a[s * kPer + j], b[s * kPer + j], x);
+        y = fma(c[s * kPer + j], d[s * kPer + j], y);
+      }
+      total += has[s] ? x.sum() + y.sum() : 0.f;
+    }
+    return total;
+  }
+  // pairs back to the order of the elements
+  static __device__ __forceinline__ void elements(const P (&a)[kPacks], const P (&b)[kPacks], float (&e)[16]) {
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      const int at = 2 * V * slot(j), i = j * W % V;
+      float t[2], u[2];
+      a[j].to(t);
+      b[j].to(u);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        e[at + (kHalf ? i + k : 2 * (i + k))] = t[k];
+        e[at + (kHalf ? V + i + k : 2 * (i + k) + 1)] = u[k];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* y, const P (&a)[kPacks], const P (&b)[kPacks]) const {
+    float e[16];
+    elements(a, b, e);
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       if (has[s]) {
@@ -217,7 +312,7 @@ struct LaneView {
     }
   }
   // cosines and sines (times sign) of the lane's pairs for the token at (b, l); 1 and 0 for those that stay
-  __device__ __forceinline__ void angles(const RotParams& p, int lane, int64_t b, int64_t l, float (&c)[8], float (&sn)[8]) const {
+  __device__ __forceinline__ void angles(const RotParams& p, int lane, int64_t b, int64_t l, float sign, float (&c)[8], float (&sn)[8]) const {
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       const int p0 = (lane + s * p.group) * V;
@@ -233,34 +328,27 @@ struct LaneView {
           const uint32_t a = min((uint32_t)__ldg(p.axis + p0 + i), (uint32_t)(p.axes - 1));   // never outside the positions
           const int64_t j = at + (int64_t)a * p.pos_sa;
           const int64_t pos = p.pos_i64 ? __ldg(static_cast<const long long*>(p.pos) + j) : (int64_t)__ldg(static_cast<const int*>(p.pos) + j);
-          const float2 cs = turn_cos_sin((uint64_t)pos * __ldg(reinterpret_cast<const unsigned long long*>(p.turns) + p0 + i));
+          const float2 cs = turn_cos_sin<sizeof(T) == 4>((uint64_t)pos * __ldg(reinterpret_cast<const unsigned long long*>(p.turns) + p0 + i));
           c[V * s + i] = cs.x;
-          sn[V * s + i] = cs.y * p.sign;
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ void turn(float (&e)[16], const float (&c)[8], const float (&sn)[8], float sign) const {
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s) {
-      if (turns[s]) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int ia = 2 * V * s + (kHalf ? i : 2 * i), ib = 2 * V * s + (kHalf ? V + i : 2 * i + 1);
-          const float a = e[ia], b = e[ib], k = c[V * s + i], t = sn[V * s + i] * sign;
-          e[ia] = a * k - b * t;
-          e[ib] = a * t + b * k;
+          sn[V * s + i] = cs.y * sign;
         }
       }
     }
   }
 };
-
 // Forward (and the plain rotation's backward).  A warp works on 32 / group tokens and one chunk of
-// their heads; kBatch heads are in flight per lane.
+// their heads; kBatch heads are in flight per lane, each one's registers are loaded again as soon as it is
+// unpacked.  Blocks in the order of the tokens, not persistent: what runs at one time then touches one
+// stretch of memory (an even share of far-apart stretches for each resident warp took 271 instead of 204 us on
+// 65536 tokens).  With the norm the weights are multiplied into the
+// cosines and sines once per token and tensor, y = r (x_a (w_a c) - x_b (w_b s), x_a (w_a s) + x_b (w_b c)), six packed
+// instructions for two pairs.
 template <typename T, int V, bool kHalf, bool kNorm>
-__global__ void __launch_bounds__(kRotThreads, 2) qk_rotary_kernel(const RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, 4) qk_rotary_kernel(const RotParams p) {
   constexpr int kBatch = sizeof(T) == 4 ? 2 : V == 1 ? 2 : 4;      // 32 registers of raw vectors
+  using View = LaneView<T, V, kHalf>;
+  using P = typename View::P;
+  constexpr int N = View::kPacks;
   const int lane = threadIdx.x & (p.group - 1);
   const int per_warp = 32 >> p.log_group;
   const int64_t unit = (int64_t)blockIdx.x * kRotWarps + (threadIdx.x >> 5);
@@ -270,9 +358,9 @@ __global__ void __launch_bounds__(kRotThreads, 2) qk_rotary_kernel(const RotPara
   if (tb * per_warp >= p.n) return;                       // the whole warp
   const bool token_live = n < p.n;
   const int64_t nn = token_live ? n : p.n - 1, b = nn / p.tokens, l = nn - b * p.tokens;
-  LaneView<T, V, kHalf> view;
+  View view;
   view.init(p, lane);
-  float c[8], sn[8];
+  float cf[8], sf[8];
   bool have_angles = false;
   const int h0 = chunk * p.chunk, h1 = h0 + p.chunk;      // heads of the chunk, keys behind the queries
 #pragma unroll
@@ -280,39 +368,64 @@ __global__ void __launch_bounds__(kRotThreads, 2) qk_rotary_kernel(const RotPara
     const int shift = which == 0 ? 0 : p.heads[0];
     const int first = max(h0 - shift, 0), last = min(h1 - shift, p.heads[which]);
     if (first >= last) continue;                          // warp-uniform
-    const T* x = static_cast<const T*>(p.x[which].p) + b * p.x[which].sb + l * p.x[which].st;
-    T* y = static_cast<T*>(p.y[which].p) + b * p.y[which].sb + l * p.y[which].st;
-    typename LaneView<T, V, kHalf>::Head raw[kBatch];
-    float w[16];
+    const int64_t xs = p.x[which].sh, ys = p.y[which].sh;
+    const T* x = static_cast<const T*>(p.x[which].p) + b * p.x[which].sb + l * p.x[which].st + first * xs;
+    T* y = static_cast<T*>(p.y[which].p) + b * p.y[which].sb + l * p.y[which].st + first * ys;
+    typename View::Head raw[kBatch];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) view.load(x + (first + u) * p.x[which].sh, token_live && first + u < last, raw[u]);
+    for (int u = 0; u < kBatch; ++u) view.load(x + min(u, last - 1 - first) * xs, raw[u]);
     if (!have_angles) {
-      view.angles(p, lane, b, l, c, sn);
+      view.angles(p, lane, b, l, p.sign, cf, sf);
       have_angles = true;
     }
-    if (kNorm) view.load_weight(p.w[which], w);
-    for (int h = first;;) {
+    // the four factors of a pair: y_a = x_a ka - x_b kb, y_b = x_a la + x_b lb
+    P ka[N], kb[N], la[N], lb[N];
+    if constexpr (kNorm) view.load_weight(p.w[which], ka, kb);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const P c = P::of(cf + j * View::W), sn = P::of(sf + j * View::W), minus = P::all(-1.f);
+      if constexpr (kNorm) {
+        const P wa = ka[j], wb = kb[j];
+        ka[j] = mul(wa, c);
+        la[j] = mul(wa, sn);
+        kb[j] = mul(mul(wb, sn), minus);
+        lb[j] = mul(wb, c);
+      } else {
+        ka[j] = lb[j] = c;
+        la[j] = sn;
+        kb[j] = mul(sn, minus);
+      }
+    }
+    for (int h = first; h < last; h += kBatch) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         if (h + u < last) {                               // warp-uniform
-          float e[16];
-          view.expand(raw[u], e);
-          if (kNorm) {
-            float sq = 0.f;
+          P a[N], d[N];
+          view.expand(raw[u], a, d);
+          P r = P::all(1.f);
+          if constexpr (kNorm) r = P::all(rsqrtf(group_sum(view.sum_of_products(a, a, d, d), p.group) * p.inv_dim + p.eps));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sq = fmaf(e[i], e[i], sq);
-            const float r = rsqrtf(group_sum(sq, p.group) * p.inv_dim + p.eps);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) e[i] = (e[i] * r) * w[i];
+          for (int j = 0; j < N; ++j) {
+            P ya = a[j], yb = d[j];
+            if (view.turns[View::slot(j)]) {
+              ya = fma(d[j], kb[j], mul(a[j], ka[j]));
+              yb = fma(d[j], lb[j], mul(a[j], la[j]));
+            } else if constexpr (kNorm) {                 // c = 1: the factors are the weights
+              ya = mul(a[j], ka[j]);
+              yb = mul(d[j], lb[j]);
+            }
+            a[j] = kNorm ? mul(ya, r) : ya;
+            d[j] = kNorm ? mul(yb, r) : yb;
           }
-          view.turn(e, c, sn, 1.f);
-          if (token_live) view.store(y + (h + u) * p.y[which].sh, e);
+          if (token_live) view.store(y + u * ys, a, d);
         }
       }
-      h += kBatch;
-      if (h >= last) break;
+      x += kBatch * xs;
+      y += kBatch * ys;
+      if (h + kBatch < last) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) view.load(x + (h + u) * p.x[which].sh, token_live && h + u < last, raw[u]);
+      for (int u = 0; u < kBatch; ++u) view.load(x + min(u, last - 1 - h - kBatch) * xs, raw[u]);
+      }
     }
   }
 }
@@ -320,7 +433,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) qk_rotary_kernel(const RotPara
 // Norm backward.  A block works on one of the tensors, so that a lane's weight gradients are 16 registers;
 // persistent: they are kept over all its tokens and reduced once.
 template <typename T, int V, bool kHalf>
-__global__ void __launch_bounds__(kRotThreads, 2) qk_norm_rotary_bwd_kernel(const RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, 4) qk_norm_rotary_bwd_kernel(const RotParams p) {
   constexpr int kBatch = sizeof(T) == 4 || V == 1 ? 1 : 2;         // 32 registers of raw vectors
   __shared__ float red[kRotMaxDim];
   const int which = (int)blockIdx.x < p.blocks0 ? 0 : 1;
@@ -331,12 +444,18 @@ __global__ void __launch_bounds__(kRotThreads, 2) qk_norm_rotary_bwd_kernel(cons
   const int heads = p.heads[which];
   const int lane = threadIdx.x & (p.group - 1), warp = threadIdx.x >> 5;
   const int per_warp = 32 >> p.log_group;
-  LaneView<T, V, kHalf> view;
+  using View = LaneView<T, V, kHalf>;
+  using P = typename View::P;
+  constexpr int N = View::kPacks;
+  View view;
   view.init(p, lane);
-  float w[16], dw[16];
-  view.load_weight(p.w[which], w);
+  // the weights wait in shared memory: their registers hold a second head's vectors instead
+  __shared__ __align__(16) float ws[kRotMaxDim];
+  for (int i = threadIdx.x; i < p.dim; i += kRotThreads) ws[i] = p.w[which][i];
+  __syncthreads();
+  P dwa[N], dwb[N];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
+  for (int j = 0; j < N; ++j) dwa[j] = dwb[j] = P::all(0.f);
   const int chunks = (heads + p.chunk - 1) / p.chunk;
   const int64_t units = (p.n + per_warp - 1) / per_warp * chunks;
   for (int64_t unit = (int64_t)block * kRotWarps + warp; unit < units; unit += (int64_t)blocks * kRotWarps) {
@@ -345,56 +464,82 @@ __global__ void __launch_bounds__(kRotThreads, 2) qk_norm_rotary_bwd_kernel(cons
     const int64_t n = tb * per_warp + ((threadIdx.x & 31) >> p.log_group);
     const bool live = n < p.n;
     const int64_t nn = live ? n : p.n - 1, b = nn / p.tokens, l = nn - b * p.tokens;
-    const T* x = static_cast<const T*>(px.p) + b * px.sb + l * px.st;
-    const T* g = static_cast<const T*>(pg.p) + b * pg.sb + l * pg.st;
-    T* y = static_cast<T*>(py.p) + b * py.sb + l * py.st;
-    typename LaneView<T, V, kHalf>::Head raw_x[kBatch], raw_g[kBatch];
-    float c[8], sn[8];
+    const T* x = static_cast<const T*>(px.p) + b * px.sb + l * px.st + first * px.sh;
+    const T* g = static_cast<const T*>(pg.p) + b * pg.sb + l * pg.st + first * pg.sh;
+    T* y = static_cast<T*>(py.p) + b * py.sb + l * py.st + first * py.sh;
+    typename View::Head raw_x[kBatch], raw_g[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      view.load(x + (first + k) * px.sh, live && first + k < last, raw_x[k]);
-      view.load(g + (first + k) * pg.sh, live && first + k < last, raw_g[k]);
+      view.load(x + min(k, last - 1 - first) * px.sh, raw_x[k]);
+      view.load(g + min(k, last - 1 - first) * pg.sh, raw_g[k]);
     }
-    view.angles(p, lane, b, l, c, sn);
-    for (int h = first;;) {
+    P c[N], sn[N];
+    {
+      float cf[8], sf[8];
+      view.angles(p, lane, b, l, -1.f, cf, sf);           // back
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        c[j] = P::of(cf + j * View::W);
+        sn[j] = P::of(sf + j * View::W);
+      }
+    }
+    for (int h = first; h < last; h += kBatch) {
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        if (h + k < last) {                               // warp-uniform; a dead token's vectors are zero
-          float e[16], u[16];
-          view.expand(raw_x[k], e);
-          view.expand(raw_g[k], u);
-          float sq = 0.f;
+        if (h + k < last) {                               // warp-uniform
+          P xa[N], xb[N], ga[N], gb[N];
+          view.expand(raw_x[k], xa, xb);
+          view.expand(raw_g[k], ga, gb);
+          const float r = rsqrtf(group_sum(view.sum_of_products(xa, xa, xb, xb), p.group) * p.inv_dim + p.eps);
+          // t = r R(-angle) dy;  dw += t x;  u = t w;  dx = u - x r^2 mean(u x)
+          const P rr = P::all(r), minus = P::all(-1.f);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sq = fmaf(e[i], e[i], sq);
-          const float r = rsqrtf(group_sum(sq, p.group) * p.inv_dim + p.eps);
-          view.turn(u, c, sn, -1.f);
-          float dot = 0.f;
-          if (live) {                                     // (a dead token's r may be infinite)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              e[i] *= r;                               // xh
-              dw[i] = fmaf(u[i], e[i], dw[i]);
-              u[i] *= w[i];
-              dot = fmaf(u[i], e[i], dot);
+          for (int j = 0; j < N; ++j) {
+            if (view.turns[View::slot(j)]) {
+              const P ta = fma(mul(gb[j], minus), sn[j], mul(ga[j], c[j]));
+              gb[j] = fma(gb[j], c[j], mul(ga[j], sn[j]));
+              ga[j] = ta;
+            }
+            ga[j] = mul(ga[j], rr);
+            gb[j] = mul(gb[j], rr);
+            if (live) {                                   // a group behind the last token repeats it and adds nothing
+              dwa[j] = fma(ga[j], xa[j], dwa[j]);
+              dwb[j] = fma(gb[j], xb[j], dwb[j]);
             }
           }
-          dot = group_sum(dot, p.group) * p.inv_dim;
-          if (live) {
+          {
+            P wa[N], wb[N];
+            view.load_weight(ws, wa, wb);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = r * (u[i] - e[i] * dot);
-            view.store(y + (h + k) * py.sh, u);
+            for (int j = 0; j < N; ++j) {
+              ga[j] = mul(ga[j], wa[j]);
+              gb[j] = mul(gb[j], wb[j]);
+            }
           }
+          const float dot = group_sum(view.sum_of_products(ga, xa, gb, xb), p.group) * p.inv_dim;
+          const P f = P::all(-r * r * dot);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            ga[j] = fma(xa[j], f, ga[j]);
+            gb[j] = fma(xb[j], f, gb[j]);
+          }
+          if (live) view.store(y + k * py.sh, ga, gb);
         }
       }
-      h += kBatch;
-      if (h >= last) break;
+      x += kBatch * px.sh;
+      g += kBatch * pg.sh;
+      y += kBatch * py.sh;
+      if (h + kBatch < last) {
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        view.load(x + (h + k) * px.sh, live && h + k < last, raw_x[k]);
-        view.load(g + (h + k) * pg.sh, live && h + k < last, raw_g[k]);
+          view.load(x + min(k, last - 1 - h - kBatch) * px.sh, raw_x[k]);
+          view.load(g + min(k, last - 1 - h - kBatch) * pg.sh, raw_g[k]);
+      }
       }
     }
   }
+  float dw[16];
+  View::elements(dwa, dwb, dw);
   // The block's weight gradients: the groups of a warp by shuffles, the warps in warp order, then one
   // row of the workspace -- a fixed association, whatever the scheduling.
 #pragma unroll
@@ -562,9 +707,7 @@ int run(const char* name, int mode, const fp4t_heads_t* x, const fp4t_heads_t* d
     ++p.log_group;
   }
   // A token's heads go to one group unless that leaves warps short of eight per SM (about the number that
-  // hides the loads' latency); then they are dealt out, down to one head per group.  (Dealing out further, to
-  // even out the last round of blocks, costs more in repeated angles than it gives: 32768 tokens with norms 124 ->
-  // 137 us.)
+  // hides the loads' latency); then they are dealt out, down to one head per group.
   const int per_warp = 32 >> p.log_group;
   const int64_t token_warps = ceil_div(p.n, per_warp);
   const auto chunk_for = [&](int heads) { return (int)ceil_div(heads, std::min<int64_t>(heads, ceil_div(8ll * sms, token_warps))); };

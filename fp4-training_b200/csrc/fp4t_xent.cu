@@ -129,16 +129,17 @@ __device__ __forceinline__ uint64_t xent_desc(uint32_t lo, int k16) {
 }
 
 // kProduct's K splits follow the number of slots too: over the clusters that its tiles leave idle, if those
-// are at least half, into pieces of two stages or more.  splits * m_tiles * n_tiles <= clusters, which
-// bounds the slices.
+// are at least half, into pieces of kMinSplitStages or more (fewer stages take less than the kernel that
+// adds the slices).  splits * m_tiles * n_tiles <= clusters, which bounds the slices.
+constexpr int kMinSplitStages = 8;
 struct SlotSplit {
   int splits, ks_per_split;
 };
 __host__ __device__ __forceinline__ SlotSplit split_slots(int m_tiles, int n_tiles, int k_stages, int clusters) {
   const int tiles = m_tiles * n_tiles;
   SlotSplit r{1, k_stages};
-  if (tiles > 0 && (int64_t)m_tiles * n_tiles * 2 <= clusters && k_stages >= 4) {
-    const int s = min(clusters / tiles, k_stages / 2);
+  if (tiles > 0 && (int64_t)m_tiles * n_tiles * 2 <= clusters) {
+    const int s = min(clusters / tiles, k_stages / kMinSplitStages);
     if (s >= 2) {
       r.ks_per_split = (k_stages + s - 1) / s;
       r.splits = (k_stages + r.ks_per_split - 1) / r.ks_per_split;
@@ -1064,8 +1065,8 @@ Cut cut_product(int64_t m, int64_t n, int64_t k, int clusters) {
   c.bn = width_for(n);
   const int64_t tiles = mt * ceil_div(n, c.bn);
   c.ks_per_split = (int)stages;
-  if (tiles * 2 <= clusters && stages >= 4) {
-    int64_t s = std::min<int64_t>(clusters / tiles, stages / 2);
+  if (tiles * 2 <= clusters) {
+    const int64_t s = std::min<int64_t>(clusters / tiles, stages / kMinSplitStages);
     if (s >= 2) {
       c.ks_per_split = (int)ceil_div(stages, s);
       c.splits = (int)ceil_div(stages, c.ks_per_split);
@@ -1321,7 +1322,7 @@ BackwardPlan plan_backward(int64_t tokens, int64_t dim, int64_t vocab, bool want
   p.ld = std::min(p.piece, round_up(vocab, 8));
   p.dw = cut_product(std::min(p.piece, vocab), dim, tokens, clusters);
   const int64_t dh_tiles = ceil_div(dim, width_for(dim));
-  p.dh_slice_rows = want_dh && dh_tiles * 2 <= clusters && ceil_div(std::min(p.piece, vocab), kXK) >= 4 ? clusters / dh_tiles * kXM : 0;
+  p.dh_slice_rows = want_dh && dh_tiles * 2 <= clusters && ceil_div(std::min(p.piece, vocab), kXK) >= 2 * kMinSplitStages ? clusters / dh_tiles * kXM : 0;
   p.o_dl = p.slots.bytes;
   p.o_acc = p.o_dl + round_up(tokens * p.ld * 2, 1024);
   p.o_cols = p.o_acc + (want_dh && p.pieces > 1 ? round_up(tokens * dim * 4, 1024) : 0);

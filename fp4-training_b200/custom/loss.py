@@ -27,17 +27,22 @@ def _operand(t, name):
     raise ValueError(f"linear_cross_entropy: {name} is {t.dtype}; it takes bfloat16 (float32 too under bfloat16 autocast)")
 
 
+def _forward(hidden, weight, bias, target, ignore_index, reduction):
+    h, w, t = _operand(hidden, "hidden"), _operand(weight, "weight"), target
+    if hidden.ndim != 2:
+        h, t = h.reshape(-1, hidden.shape[-1]), target.reshape(-1)
+    loss, lse, _ = _ops.linear_cross_entropy_forward(h, w, bias, t, ignore_index, reduction)
+    return h, w, t, loss.view(target.shape) if reduction == "none" else loss, lse
+
+
 class _LinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, target, ignore_index, reduction):
         ctx.dtypes = hidden.dtype, weight.dtype, None if bias is None else bias.dtype
         ctx.shape, ctx.args = hidden.shape, (ignore_index, reduction)
-        h = _operand(hidden.reshape(-1, hidden.shape[-1]), "hidden")
-        w = _operand(weight, "weight")
-        t = target.reshape(-1)
-        loss, lse, _ = _ops.linear_cross_entropy_forward(h, w, bias, t, ignore_index, reduction)
+        h, w, t, loss, lse = _forward(hidden, weight, bias, target, ignore_index, reduction)
         ctx.save_for_backward(h, w, bias, t, lse)
-        return loss.view(target.shape) if reduction == "none" else loss
+        return loss
 
     @staticmethod
     @once_differentiable
@@ -45,7 +50,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         h, w, bias, t, lse = ctx.saved_tensors
         want = [dt if need else None for dt, need in zip(ctx.dtypes, ctx.needs_input_grad)]
         dh, dw, db = _ops.linear_cross_entropy_backward(grad.reshape(-1), h, w, bias, t, lse, *ctx.args, *want)
-        return None if dh is None else dh.view(ctx.shape), dw, db, None, None, None
+        return None if dh is None else dh.view(ctx.shape), dw, db, None, None, None     # (a head frozen in training: only dh)
 
 
 def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, reduction="mean"):
@@ -57,7 +62,9 @@ def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, r
     if hidden.ndim < 1 or weight.ndim != 2 or target.shape != hidden.shape[:-1]:
         raise ValueError("linear_cross_entropy takes hidden [..., D], weight [V, D] and target [...], got "
                          f"{tuple(hidden.shape)}, {tuple(weight.shape)} and {tuple(target.shape)}")
-    return _LinearCrossEntropyFn.apply(hidden, weight, bias, target, int(ignore_index), reduction)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LinearCrossEntropyFn.apply(hidden, weight, bias, target, int(ignore_index), reduction)
+    return _forward(hidden, weight, bias, target, int(ignore_index), reduction)[3]
 
 
 class LinearCrossEntropy(nn.Module):

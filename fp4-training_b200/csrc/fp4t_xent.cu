@@ -11,8 +11,12 @@
 //             that a small kernel joins along the vocabulary;
 //   backward  in pieces of the vocabulary: the logits of a piece are computed again, turned into dl in
 //             the epilogue and written once, in bf16 (the operand type of the two products that read
-//             it; a rounding of 2^-9 on average per term, as large as the one that dh and dW get at the end);
-//             dh accumulates over the pieces in fp32, dW's rows of the piece are final.
+//             it); dh accumulates over the pieces in fp32, dW's rows of the piece are final.
+//             That rounding is off by half a step, 2^-8, per term at most, as the one that dh and dW get at the
+//             end, and at many tokens as independent.  A scalar g_t is kept out of it (it scales the products'
+//             epilogues): rounded into every term it would be one error in all of them.  Up to 64 tokens, where a
+//             few roundings do not average out, dl is kept as a sum of two bf16, rows 64 to 127 holding
+//             what rows 0 to 63 lost; the tiles are 256 rows high and wait for W, so this costs no time.
 // Recomputing costs 2 T V D operations on top of the 6 T V D that cannot be avoided, and saves the
 // T x V logits (4 GB of fp32 at 8192 x 131072).
 //
@@ -40,13 +44,14 @@ constexpr int kXM = 256, kXK = 64;               // rows and K elements of a til
 constexpr int kXEpiWarps = 8;
 constexpr int kXThreads = 128 + 32 * kXEpiWarps; // producer, MMA issuer, tensor-memory owner, an idle warp, epilogue
 constexpr int kXTmemCols = 512;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Logits are scaled by log2(e) in the multiply-add that subtracts the maximum.  A maximum (or lse) beyond
 // this would overflow there -- a row masked with the type's lowest value, or infinite -- and is
 // subtracted first instead.
 constexpr float kFar = 2e38f;
 constexpr int kXBadTarget = 41;                  // status: a target outside the vocabulary
 
+constexpr int kFew = 64;                         // tokens up to which dl is kept in two bf16 (one K stage)
 constexpr int64_t kTokenBlock = 16384;           // tokens whose partial statistics are held at once
 constexpr int64_t kPieceBytes = 512ll << 20;     // dl of one piece of the vocabulary, unless that makes
 constexpr int64_t kMinPiece = 4096;              // the piece narrower than this
@@ -59,6 +64,7 @@ struct XParams {
   const int* slots;                              // number of counted tokens
   int tokens;                                    // all tokens: slots == tokens means that h can be read as it is
   int slot0;                                     // kStats: first slot of the block
+  int few;                                       // backward, at most kFew tokens: dl has 2 kFew rows, h is packed twice
   int split_clusters;                            // kProduct: clusters that K may be split over (0: it may not)
   // kStats, kGrad
   const void* bias;
@@ -70,7 +76,7 @@ struct XParams {
   const float* lse;
   const float* grad;
   int grad_per_row;
-  int mean;                                      // kGrad: divide by the number of counted tokens
+  int mean;                                      // divide by the number of counted tokens
   const int* token;                              // slot -> token (grad_per_row, and kProduct's rows)
   float* col_part;                               // kGrad: column sums of dl over 32 slots, [slots / 32][col_ld], or null
   int64_t col_ld;
@@ -336,12 +342,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 
   // The work follows the number of counted tokens: rows of the output, or the length of K.
   const int slots = *static_cast<const volatile int*>(g.slots);
-  const bool dense = slots == g.tokens;
+  const bool dense = slots == g.tokens && !g.few;
+  const int dl_rows = g.few ? 2 * kFew : slots;
   if (kMode == kProductT) {
-    g.k_stages = (slots + kXK - 1) / kXK;
+    g.k_stages = (dl_rows + kXK - 1) / kXK;
     g.ks_per_split = (g.k_stages + g.splits - 1) / g.splits;
   } else {
-    g.rows = max(0, min(g.rows, slots - g.slot0));
+    g.rows = max(0, min(g.rows, dl_rows - g.slot0));
     g.m_tiles = (g.rows + kXM - 1) / kXM;
     if (kMode == kProduct && g.split_clusters > 0) {
       const SlotSplit sp = split_slots(g.m_tiles, g.n_tiles, g.k_stages, g.split_clusters);
@@ -350,7 +357,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       g.slice_rows = g.m_tiles * kXM;
     }
   }
-  const bool sliced = kMode == kProduct && g.splits > 1;      // fp32 slices (map_packed), summed by another kernel
+  const bool sliced = kMode == kProduct && (g.splits > 1 || g.few);   // fp32 slices (map_packed), summed by another kernel
   const CUtensorMap* tma_a = (kMode == kStats || kMode == kGrad) && !dense ? &map_packed : &map_a;
   const CUtensorMap* tma_b = kMode == kProductT && !dense ? &map_packed : &map_b;
   const int units = g.m_tiles * g.n_tiles * g.splits;
@@ -437,8 +444,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int quad = warp & 3, half = (warp - 4) >> 2;
     uint8_t* buf = smem + C::kEpi0 + (warp - 4) * 4096;
     uint32_t n_emit = 0;
-    float scale = 0.f;
-    if (kMode == kGrad && !g.grad_per_row) scale = g.mean ? __ldg(g.grad) / (float)slots : __ldg(g.grad);
+    // a scalar gradient of the loss scales the products (and db), one per token is part of dl
+    float scale = 1.f;
+    if (kMode != kStats && !g.grad_per_row) scale = g.mean ? (slots > 0 ? __ldg(g.grad) / (float)slots : 0.f) : __ldg(g.grad);
     int it = 0;
     for (int unit = cluster_id; unit < units; unit += num_clusters, ++it) {
       const TilePos t = tile_at(g, unit);
@@ -450,7 +458,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       tc_fence_after();
       const uint32_t acc = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(a * kBN + half * C::kHalf);
       const int row0 = t.m * kXM + (int)rank * 128 + quad * 32, row = row0 + lane;
-      const bool row_ok = row < g.rows;
+      const int slot = kMode == kGrad && g.few ? row & (kFew - 1) : row;
+      const bool row_ok = row < g.rows && (kMode != kGrad || slot < slots);
       const int colbase = t.n * kBN + half * C::kHalf;
       auto release = [&]() {
         tc_fence_before();
@@ -459,15 +468,15 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       };
       if (kMode == kStats || kMode == kGrad) {
         // the target's column in this warp's part of the tile; anything outside [0, cols) never matches
-        const int yc = row_ok ? __ldg(g.target + row) - g.col0 : -1;
+        const int yc = row_ok ? __ldg(g.target + slot) - g.col0 : -1;
         const int mine = yc >= colbase && yc < colbase + C::kHalf && yc < g.cols ? yc - colbase : -1;
         // dl's rows up to the end of the last K stage that reads them are written (as zeros)
         const int row_end = kMode == kGrad ? (g.rows + kXK - 1) / kXK * kXK : g.rows;
         float m = -INFINITY, s = 0.f, x_y = 0.f;
         float lse = 0.f, gr = 0.f;
         if (kMode == kGrad) {
-          lse = row_ok ? __ldg(g.lse + row) : 0.f;
-          gr = g.grad_per_row ? (row_ok ? __ldg(g.grad + __ldg(g.token + row)) : 0.f) : scale;
+          lse = row_ok ? __ldg(g.lse + slot) : 0.f;
+          gr = g.grad_per_row ? (row_ok ? __ldg(g.grad + __ldg(g.token + slot)) : 0.f) : 1.f;
         }
 #pragma unroll 1
         for (int c = 0; c < C::kHalf / 32; ++c) {
@@ -506,7 +515,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 s2 += exp2_fast(fmaf(v[j + 2], kLog2e, -ref));
                 s3 += exp2_fast(fmaf(v[j + 3], kLog2e, -ref));
               }
-              s = fmaf(s, exp2_fast(fmaf(m, kLog2e, -ref)), (s0 + s1) + (s2 + s3));
+              // ref is mn log2(e) rounded, the same error in all terms: the residual takes it out of their sum
+              s = fmaf(s, exp2_fast((m - mn) * kLog2e), ((s0 + s1) + (s2 + s3)) * fmaf(fmaf(mn, kLog2e, -ref), -kLn2, 1.f));
             } else {
               const float ref = mn == -INFINITY ? 0.f : mn;           // a row of -inf so far: all terms are 0
               float s0 = 0.f;
@@ -531,9 +541,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = row_ok ? v[j] * gr : 0.f;
-            if (g.col_part != nullptr) {
-              const float sum = column_sums(v, lane);
+            if (g.col_part != nullptr && (!g.few || row0 < kFew)) {
+              const float sum = column_sums(v, lane) * scale;
               if (col + lane < g.cols) g.col_part[(int64_t)(row0 >> 5) * g.col_ld + col + lane] = sum;
+            }
+            if (g.few && row0 >= kFew) {                      // what the rows' first bf16 lose
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
             }
             store_chunk_bf16(&map_d, buf, n_emit, lane, row0, col, v);
           }
@@ -557,7 +571,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           if (col >= g.cols || row0 >= g.rows) continue;
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = nothing ? 0.f : __uint_as_float(r[j]);
+          for (int j = 0; j < 32; ++j) v[j] = nothing ? 0.f : __uint_as_float(r[j]) * scale;
           if (g.acc != nullptr && row_ok && !sliced) {         // columns are a multiple of 8: whole vectors
             const float4* p = reinterpret_cast<const float4*>(g.acc + (int64_t)row * g.ldacc + col);
 #pragma unroll
@@ -604,7 +618,8 @@ struct PackParams {
   const __nv_bfloat16* h;
   int64_t ldh;
   int dim;
-  __nv_bfloat16* packed;                         // [tokens][dim]
+  __nv_bfloat16* packed;                         // [tokens][dim]; few: [2 kFew][dim], the rows twice
+  int few;
   int* slots;
   int* token;                                    // slot -> token
   int* slot_target;
@@ -659,7 +674,7 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
   }
   all = pack_block_sum(all, red);
   before = pack_block_sum(before, red);
-  const bool dense = all == p.tokens;
+  const bool dense = all == p.tokens && !p.few;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     *p.slots = all;
     if (p.counter) *p.counter = 0u;
@@ -698,7 +713,10 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
             if (c0 + 32 * k < p.dim / 8) v[k] = __ldg(from + c0 + 32 * k);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (c0 + 32 * k < p.dim / 8) to[c0 + 32 * k] = v[k];
+            if (c0 + 32 * k < p.dim / 8) {
+              to[c0 + 32 * k] = v[k];
+              if (p.few) to[c0 + 32 * k + (int64_t)kFew * (p.dim / 8)] = v[k];
+            }
         }
       }
       if (p.dh != nullptr) {
@@ -716,9 +734,11 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
   }
   // the rows behind the last slot that the last K stage of dW reads are zero
   if (!dense && blockIdx.x == gridDim.x - 1) {
-    const int end = min(p.tokens, (all + kXK - 1) / kXK * kXK);
-    for (int64_t c = (int64_t)all * (p.dim / 8) + threadIdx.x; c < (int64_t)end * (p.dim / 8); c += kPackThreads)
+    const int end = p.few ? kFew : min(p.tokens, (all + kXK - 1) / kXK * kXK);
+    for (int64_t c = (int64_t)all * (p.dim / 8) + threadIdx.x; c < (int64_t)end * (p.dim / 8); c += kPackThreads) {
       reinterpret_cast<uint4*>(p.packed)[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (p.few) reinterpret_cast<uint4*>(p.packed)[c + (int64_t)kFew * (p.dim / 8)] = make_uint4(0u, 0u, 0u, 0u);
+    }
   }
 }
 
@@ -908,10 +928,10 @@ __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const JoinParam
   double sum = 0.0;
   if (slice == 0 && row < rows) {
     const float2 q = red[threadIdx.x];
-    const float lse = q.x + logf(q.y);
-    p.lse[row] = lse;
+    const double lse = (double)q.x + (double)logf(q.y);      // the loss is a small difference of large numbers
+    p.lse[row] = (float)lse;
     float loss = NAN;
-    if (p.target[row] >= 0) loss = lse - p.picked[row];
+    if (p.target[row] >= 0) loss = (float)(lse - (double)p.picked[row]);
     else if (p.status) atomicCAS(p.status, 0, kXBadTarget);
     if (p.row_loss) p.row_loss[p.token[row]] = loss;
     sum = loss;
@@ -952,6 +972,7 @@ struct SliceParams {
   const int* slots;                      // dh: the splits are kProduct's own
   const int* token;
   int n_tiles, k_stages, split_clusters;
+  int few;                               // dh: rows kFew further on are added
 };
 __global__ void __launch_bounds__(256) xent_slices_kernel(const SliceParams p) {
   pdl_launch_dependents();
@@ -962,9 +983,9 @@ __global__ void __launch_bounds__(256) xent_slices_kernel(const SliceParams p) {
   if (p.slots != nullptr) {
     rows = min(rows, *static_cast<const volatile int*>(p.slots));
     scatter = p.token != nullptr && rows < p.tokens;
-    const int m_tiles = (rows + kXM - 1) / kXM;
+    const int m_tiles = p.few ? 1 : (rows + kXM - 1) / kXM;
     n = split_slots(m_tiles, p.n_tiles, p.k_stages, p.split_clusters).splits;
-    if (n == 1) return;                  // written by kProduct itself
+    if (n == 1 && !p.few) return;        // written by kProduct itself
     slice_elems = (int64_t)m_tiles * kXM * p.cols4 * 4;
   }
   const int64_t total4 = (int64_t)rows * p.cols4;
@@ -973,6 +994,10 @@ __global__ void __launch_bounds__(256) xent_slices_kernel(const SliceParams p) {
     for (int s = 0; s < n; ++s) {
       const float4 f = reinterpret_cast<const float4*>(p.slices + s * slice_elems)[i];
       v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+      if (p.few) {
+        const float4 l = reinterpret_cast<const float4*>(p.slices + s * slice_elems)[i + (int64_t)kFew * p.cols4];
+        v.x += l.x; v.y += l.y; v.z += l.z; v.w += l.w;
+      }
     }
     int64_t to = i;
     if (scatter) {
@@ -1172,11 +1197,25 @@ struct Slots {
   __nv_bfloat16* packed;
 };
 
+// The loss's gradient as the kernels take it.
+struct Scale {
+  const float* grad;
+  int reduction;
+  void to(XParams& g) const {
+    g.grad = grad;
+    g.grad_per_row = reduction == FP4T_XENT_NONE;
+    g.mean = reduction == FP4T_XENT_MEAN;
+  }
+};
+
 // dh (or its sum over the pieces so far) into `out`, rows of `dim`: slots, or tokens' places if to_tokens.
 int run_dh(const Operand& dl, const Operand& w, int64_t tokens, int64_t dim, int64_t vc, void* out, int out_f32, bool to_tokens, const float* acc,
-           float* slices, int64_t slice_rows, int split_clusters, const Slots& sl, int32_t* status, cudaStream_t stream) {
+           float* slices, int64_t slice_rows, int split_clusters, const Scale& scale, const Slots& sl, int32_t* status, cudaStream_t stream) {
   XParams g = {};
-  g.rows = g.tokens = (int)tokens;
+  g.few = tokens <= kFew;
+  g.tokens = (int)tokens;
+  g.rows = g.few ? 2 * kFew : (int)tokens;
+  scale.to(g);
   g.cols = (int)dim;
   g.slots = sl.slots;
   g.token = sl.token;
@@ -1199,6 +1238,7 @@ int run_dh(const Operand& dl, const Operand& w, int64_t tokens, int64_t dim, int
   p.cols4 = (int)(dim / 4);
   p.slots = sl.slots;
   p.token = to_tokens ? sl.token : nullptr;
+  p.few = g.few;
   p.n_tiles = (int)ceil_div(dim, bn);
   p.k_stages = (int)ceil_div(vc, kXK);
   p.split_clusters = split_clusters;
@@ -1208,18 +1248,20 @@ int run_dh(const Operand& dl, const Operand& w, int64_t tokens, int64_t dim, int
 
 // dW's rows of a piece, through slices when it is split (few entries, many tokens).
 int run_dw(const Cut& cut, const Operand& dl, const Operand& h, const Operand& packed, int64_t tokens, int64_t dim, int64_t vc, void* out, int out_f32,
-           float* slices, const Slots& sl, int32_t* status, cudaStream_t stream) {
+           float* slices, const Scale& scale, const Slots& sl, int32_t* status, cudaStream_t stream) {
   XParams g = {};
+  g.few = tokens <= kFew;
   g.rows = (int)vc;
   g.cols = (int)dim;
   g.tokens = (int)tokens;
+  scale.to(g);
   g.slots = sl.slots;
   g.status = status;
   g.splits = cut.splits;
   g.ks_per_split = cut.ks_per_split;
   g.out_f32 = cut.splits > 1 ? 1 : out_f32;
   g.slice_rows = (int)cut.slice_rows;
-  int rc = launch_xent<kProductT>(cut.bn, dl, h, packed, cut.splits > 1 ? slices : out, dim, g, tokens, stream);
+  int rc = launch_xent<kProductT>(cut.bn, dl, h, packed, cut.splits > 1 ? slices : out, dim, g, dl.outer, stream);
   if (rc != FP4T_OK || cut.splits == 1) return rc;
   SliceParams p = {};
   p.slices = slices;
@@ -1235,9 +1277,9 @@ int run_dw(const Cut& cut, const Operand& dl, const Operand& h, const Operand& p
 
 // Slots in the workspace: their number, the token and target of each, counts per run, the packed rows of h.
 struct SlotPlan {
-  int64_t run, runs, o_token, o_target, o_runs, o_packed, bytes;
+  int64_t run, runs, o_token, o_target, o_runs, o_packed, packed_rows, bytes;
 };
-SlotPlan plan_slots(int64_t tokens, int64_t dim) {
+SlotPlan plan_slots(int64_t tokens, int64_t dim, bool backward) {
   SlotPlan p;
   p.run = round_up(ceil_div(tokens, 148 * 4), 8);        // a warp copies a row at a time, a block has eight
   p.runs = ceil_div(tokens, p.run);
@@ -1245,7 +1287,8 @@ SlotPlan plan_slots(int64_t tokens, int64_t dim) {
   p.o_target = p.o_token + round_up(tokens * 4, 128);
   p.o_runs = p.o_target + round_up(tokens * 4, 128);
   p.o_packed = round_up(p.o_runs + p.runs * 4, 1024);
-  p.bytes = p.o_packed + round_up(tokens * dim * 2, 1024);
+  p.packed_rows = backward && tokens <= kFew ? 2 * kFew : tokens;
+  p.bytes = p.o_packed + round_up(p.packed_rows * dim * 2, 1024);
   return p;
 }
 Slots slots_at(uint8_t* ws, const SlotPlan& p) {
@@ -1264,6 +1307,7 @@ int launch_pack(const SlotPlan& plan, const Slots& sl, const void* h, int64_t ld
   p.ldh = ldh;
   p.dim = (int)dim;
   p.packed = sl.packed;
+  p.few = plan.packed_rows > tokens;
   p.slots = sl.slots;
   p.token = sl.token;
   p.slot_target = sl.target;
@@ -1290,7 +1334,7 @@ struct ForwardPlan {
 };
 ForwardPlan plan_forward(int64_t tokens, int64_t dim, int64_t vocab) {
   ForwardPlan p;
-  p.slots = plan_slots(tokens, dim);
+  p.slots = plan_slots(tokens, dim, false);
   p.block = std::min(tokens, kTokenBlock);
   p.rows_blocks = tokens <= kRowsTokens && (tokens == 3 ? 4 : tokens) * dim <= kRowsElems ? std::min<int64_t>(ceil_div(vocab, kRowsThreads / 32 * kRowsPerWarp), 148 * 2) : 0;
   p.parts = p.rows_blocks > 0 ? p.rows_blocks : 2 * ceil_div(vocab, width_for(vocab));
@@ -1314,17 +1358,19 @@ struct BackwardPlan {
 };
 BackwardPlan plan_backward(int64_t tokens, int64_t dim, int64_t vocab, bool want_dh, bool want_dw, bool want_db, int clusters) {
   BackwardPlan p;
-  p.slots = plan_slots(tokens, dim);
+  p.slots = plan_slots(tokens, dim, true);
   p.piece = std::min(round_up(vocab, 256), std::max(kMinPiece, kPieceBytes / (2 * tokens) / 256 * 256));
   p.pieces = ceil_div(vocab, p.piece);
   p.piece = round_up(ceil_div(vocab, p.pieces), 256);       // even pieces
   p.pieces = ceil_div(vocab, p.piece);
   p.ld = std::min(p.piece, round_up(vocab, 8));
-  p.dw = cut_product(std::min(p.piece, vocab), dim, tokens, clusters);
+  p.dw = cut_product(std::min(p.piece, vocab), dim, p.slots.packed_rows, clusters);
   const int64_t dh_tiles = ceil_div(dim, width_for(dim));
   p.dh_slice_rows = want_dh && dh_tiles * 2 <= clusters && ceil_div(std::min(p.piece, vocab), kXK) >= 2 * kMinSplitStages ? clusters / dh_tiles * kXM : 0;
+  if (want_dh && tokens <= kFew) p.dh_slice_rows = std::max<int64_t>(p.dh_slice_rows, kXM);
+  const int64_t dl_rows = p.slots.packed_rows;
   p.o_dl = p.slots.bytes;
-  p.o_acc = p.o_dl + round_up(tokens * p.ld * 2, 1024);
+  p.o_acc = p.o_dl + round_up(dl_rows * p.ld * 2, 1024);
   p.o_cols = p.o_acc + (want_dh && p.pieces > 1 ? round_up(tokens * dim * 4, 1024) : 0);
   p.o_slices = p.o_cols + (want_db ? round_up(round_up(tokens, kXK) / 32 * p.ld * 4, 1024) : 0);
   p.bytes = p.o_slices + std::max(p.dh_slice_rows * dim * 4, want_dw ? p.dw.slice_bytes(dim) : 0);
@@ -1489,12 +1535,14 @@ extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, 
   __nv_bfloat16* dl = reinterpret_cast<__nv_bfloat16*>(ws + p.o_dl);
   float* acc = reinterpret_cast<float*>(ws + p.o_acc);
   float* slices = reinterpret_cast<float*>(ws + p.o_slices);
-  const Operand hop{h, tokens, dim, ldh}, packed{sl.packed, tokens, dim, dim};
+  const Operand hop{h, tokens, dim, ldh}, packed{sl.packed, p.slots.packed_rows, dim, dim};
+  const Scale scale{grad_loss, reduction};
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, vc = std::min(p.piece, vocab - v0);
-    const Operand wop{static_cast<const __nv_bfloat16*>(w) + v0 * ldw, vc, dim, ldw}, dop{dl, tokens, vc, p.ld};
+    const Operand wop{static_cast<const __nv_bfloat16*>(w) + v0 * ldw, vc, dim, ldw}, dop{dl, p.slots.packed_rows, vc, p.ld};
     XParams g = {};
-    g.rows = (int)tokens;
+    g.rows = (int)p.slots.packed_rows;
+    g.few = tokens <= kFew;
     g.cols = (int)vc;
     g.tokens = (int)tokens;
     g.slots = sl.slots;
@@ -1504,9 +1552,7 @@ extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, 
     g.target = sl.target;
     g.col0 = (int)v0;
     g.lse = lse;
-    g.grad = grad_loss;
-    g.grad_per_row = reduction == FP4T_XENT_NONE;
-    g.mean = reduction == FP4T_XENT_MEAN;
+    scale.to(g);
     g.col_part = db ? reinterpret_cast<float*>(ws + p.o_cols) : nullptr;
     g.col_ld = p.ld;
     g.status = status;
@@ -1515,12 +1561,12 @@ extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, 
     if (dh) {
       const bool last = i == p.pieces - 1;
       rc = run_dh(dop, wop, tokens, dim, vc, last ? dh : static_cast<void*>(acc), last ? dh_dtype == FP4T_DT_F32 : 1, last, i > 0 ? acc : nullptr,
-                  slices, p.dh_slice_rows, clusters, sl, status, s);
+                  slices, p.dh_slice_rows, clusters, scale, sl, status, s);
       if (rc != FP4T_OK) return rc;
     }
     if (dw) {
       void* out = static_cast<uint8_t*>(dw) + v0 * dim * (dw_dtype == FP4T_DT_F32 ? 4 : 2);
-      rc = run_dw(p.dw, dop, hop, packed, tokens, dim, vc, out, dw_dtype == FP4T_DT_F32, slices, sl, status, s);
+      rc = run_dw(p.dw, dop, hop, packed, tokens, dim, vc, out, dw_dtype == FP4T_DT_F32, slices, scale, sl, status, s);
       if (rc != FP4T_OK) return rc;
     }
     if (db) {

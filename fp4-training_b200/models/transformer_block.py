@@ -11,6 +11,7 @@ from custom import (
     CublasltNvfp4Linear,
     CustomLinear,
     FusedLayerNorm,
+    FusedQKNorm,
 )
 
 LINEAR_IMPL = {
@@ -32,7 +33,8 @@ class AttentionBlock(nn.Module):
     (models/transformer_block.py:74,95) attn_scale is 1 / dh**-0.5, i.e. the scores are
     MULTIPLIED by sqrt(dh); loss-curve parity depends on keeping that."""
 
-    def __init__(self, E, H, dropout=0.1, impl="torch", fused_norm=False, fuse_qkv=False, sdpa=False):
+    def __init__(self, E, H, dropout=0.1, impl="torch", fused_norm=False, fuse_qkv=False, sdpa=False, rotary=None, positions=None,
+                 qk_norm=False):
         super().__init__()
         self.fuse_qkv = fuse_qkv        # an addition: q / k / v as one quantization + one GEMM over stacked weights
         # an addition: the attention core through torch's scaled_dot_product_attention (a library
@@ -49,6 +51,23 @@ class AttentionBlock(nn.Module):
         self.v_proj = linear(E, E)
         self.o_proj = linear(E, E)
         self.dropout = nn.Dropout(dropout)
+        # additions: rotary positions (a RotaryPositions and its integer positions [L, axes]) and RMS
+        # norms of the query and key heads, both in one pass where both are asked for
+        if rotary is not None and positions is None:
+            raise ValueError("rotary positions need the tokens' positions")
+        self.rotary = None if qk_norm else rotary
+        self.qk_norm = FusedQKNorm(self.dh, rotary=rotary) if qk_norm else None
+        if qk_norm:      # the scores are multiplied by sqrt(dh) below: this makes them q k^T / sqrt(dh) of the normalised heads
+            nn.init.constant_(self.qk_norm.q_weight, 1.0 / self.dh)
+        self.register_buffer("positions", positions if rotary is not None else None, persistent=False)
+
+    def _positioned(self, q, k):
+        """q and k [B, L, H, dh] after the norm and the rotation, where the block has them."""
+        if self.qk_norm is not None:
+            return self.qk_norm(q, k, self.positions)
+        if self.rotary is not None:
+            return self.rotary(q, k, positions=self.positions)
+        return q, k
 
     def forward(self, x):
         B, L, E = x.shape
@@ -58,14 +77,15 @@ class AttentionBlock(nn.Module):
             q, k, v = self.q_proj.forward_stacked([self.q_proj, self.k_proj, self.v_proj], x)
         else:
             q, k, v = self.q_proj(x), self.k_proj(x), self.v_proj(x)
-        q = q.view(B, L, self.H, self.dh).transpose(1, 2)
+        q, k = self._positioned(q.view(B, L, self.H, self.dh), k.view(B, L, self.H, self.dh))
+        q = q.transpose(1, 2)
         if self.sdpa:
-            k = k.view(B, L, self.H, self.dh).transpose(1, 2)
+            k = k.transpose(1, 2)
             v = v.view(B, L, self.H, self.dh).transpose(1, 2)
             attn = F.scaled_dot_product_attention(q, k, v, dropout_p=self.dropout.p if self.training else 0.0,
                                                   scale=self.attn_scale)
             return residual + self.o_proj(attn.transpose(1, 2).reshape(B, L, E))
-        k_t = k.view(B, L, self.H, self.dh).transpose(1, 2).transpose(-2, -1)
+        k_t = k.transpose(1, 2).transpose(-2, -1)
         v = v.view(B, L, self.H, self.dh).transpose(1, 2)
         prob = self.dropout(F.softmax((q @ k_t) * self.attn_scale, dim=-1))
         attn = (prob @ v).transpose(1, 2).contiguous().view(B, L, E)
@@ -73,13 +93,15 @@ class AttentionBlock(nn.Module):
 
 
 class TransformerBlock(nn.Module):
-    def __init__(self, E, F, H, dropout=0.1, impl="torch", fuse_gelu=False, fused_norm=False, fuse_qkv=False, sdpa=False):
+    def __init__(self, E, F, H, dropout=0.1, impl="torch", fuse_gelu=False, fused_norm=False, fuse_qkv=False, sdpa=False,
+                 rotary=None, positions=None, qk_norm=False):
         super().__init__()
         self.E, self.F, self.H, self.impl = E, F, H, impl
         self.fuse_gelu = fuse_gelu      # an addition: see forward()
         # fused_norm (an addition): the two `preln` modules run on the library's LayerNorm kernels
         # (same parameters and state dict as nn.LayerNorm)
-        self.attn = AttentionBlock(E, H, dropout, impl=impl, fused_norm=fused_norm, fuse_qkv=fuse_qkv, sdpa=sdpa)
+        self.attn = AttentionBlock(E, H, dropout, impl=impl, fused_norm=fused_norm, fuse_qkv=fuse_qkv, sdpa=sdpa,
+                                   rotary=rotary, positions=positions, qk_norm=qk_norm)
         linear = LINEAR_IMPL[impl]
         self.ffn = nn.ModuleDict({
             "preln": FusedLayerNorm(E) if fused_norm else nn.LayerNorm(E),

@@ -32,9 +32,10 @@ from dp import GradAllReducer, broadcast_parameters  # noqa: E402
 from models import REF_IMPL, TinyViT  # noqa: E402
 
 
-def build_model(impl, depth, device, fused_norm=False, fuse_qkv=False, sdpa=False):
+def build_model(impl, depth, device, fused_norm=False, fuse_qkv=False, sdpa=False, rope=False, qk_norm=False):
     return TinyViT(img_size=28, patch_size=4, in_chans=1, num_classes=10, embed_dim=192, num_heads=3,
-                   mlp_ratio=4.0, linear_impl=impl, depth=depth, fused_norm=fused_norm, fuse_qkv=fuse_qkv, sdpa=sdpa).to(device)
+                   mlp_ratio=4.0, linear_impl=impl, depth=depth, fused_norm=fused_norm, fuse_qkv=fuse_qkv, sdpa=sdpa,
+                   rope=rope, qk_norm=qk_norm).to(device)
 
 
 def _sync(device, world):
@@ -45,7 +46,7 @@ def _sync(device, world):
 
 
 def train(impl="cublaslt_nvfp4", steps=200, warmup=5, batch=512, depth=6, seed=0, lr=1e-3, device=None, log=None,
-          fp32=False, graph=False, fused_norm=False, fuse_qkv=False, sdpa=False):
+          fp32=False, graph=False, fused_norm=False, fuse_qkv=False, sdpa=False, rope=False, qk_norm=False, fused_loss=False):
     """graph=True (CUDA only): forward + backward and the optimizer step are captured once into
     two CUDA graphs and replayed per step, with the gradient all-reduce (one NCCL call on a flat
     buffer that all `.grad` tensors are views of) between them.  The step is launch-bound at
@@ -62,9 +63,15 @@ def train(impl="cublaslt_nvfp4", steps=200, warmup=5, batch=512, depth=6, seed=0
         os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
         dist.init_process_group("nccl" if device.type == "cuda" else "gloo")
     torch.manual_seed(seed)
-    model = build_model(impl, depth, device, fused_norm, fuse_qkv, sdpa)
+    if fused_loss and (fp32 or device.type != "cuda"):
+        raise ValueError("fused_loss needs a CUDA device and bfloat16 autocast")
+    model = build_model(impl, depth, device, fused_norm, fuse_qkv, sdpa, rope, qk_norm)
     broadcast_parameters(model)
     crit = nn.CrossEntropyLoss()
+
+    def loss_of(x, y):
+        return model.loss(x, y) if fused_loss else crit(model(x), y)
+
     torch.manual_seed(seed + 1000 * (rank + 1))        # data, dropout and rounding noise differ per rank
     gen = torch.Generator(device=device).manual_seed(seed + 77 * (rank + 1))
 
@@ -94,7 +101,7 @@ def train(impl="cublaslt_nvfp4", steps=200, warmup=5, batch=512, depth=6, seed=0
             flat.zero_()
             counter.add_(1)
             with torch.autocast(device.type, dtype=torch.bfloat16, enabled=not fp32):
-                loss = crit(model(sx), sy)
+                loss = loss_of(sx, sy)
             loss.backward()
             return loss.detach()
 
@@ -140,7 +147,7 @@ def train(impl="cublaslt_nvfp4", steps=200, warmup=5, batch=512, depth=6, seed=0
                 t0 = time.perf_counter()
             x, y = batch_of()
             with torch.autocast(device.type, dtype=torch.bfloat16, enabled=not fp32):
-                loss = crit(model(x), y)
+                loss = loss_of(x, y)
             opt.zero_grad(set_to_none=True)
             loss.backward()
             reducer.finish()
@@ -154,7 +161,8 @@ def train(impl="cublaslt_nvfp4", steps=200, warmup=5, batch=512, depth=6, seed=0
             for i, v in enumerate(losses):
                 f.write(json.dumps({"step": i, "loss": v}) + "\n")
     return {"impl": impl, "steps": steps, "world": world, "batch_per_gpu": batch, "depth": depth, "graph": bool(graph),
-            "fused_norm": bool(fused_norm), "fuse_qkv": bool(fuse_qkv), "sdpa": bool(sdpa),
+            "fused_norm": bool(fused_norm), "fuse_qkv": bool(fuse_qkv), "sdpa": bool(sdpa), "rope": bool(rope),
+            "qk_norm": bool(qk_norm), "fused_loss": bool(fused_loss),
             "steps_per_s": steps / dt, "images_per_s": steps * batch * world / dt, "first_loss": losses[0],
             "last_loss": losses[-1], "losses": losses}
 
@@ -174,8 +182,12 @@ def main():
     ap.add_argument("--fused-norm", action="store_true", help="LayerNorms on the library's kernels")
     ap.add_argument("--fuse-qkv", action="store_true", help="q / k / v as one quantization and one GEMM")
     ap.add_argument("--sdpa", action="store_true", help="attention core through torch's scaled_dot_product_attention")
+    ap.add_argument("--rope", action="store_true", help="rotary positions by the patches' rows and columns")
+    ap.add_argument("--qk-norm", action="store_true", help="RMS norm of every query and key head")
+    ap.add_argument("--fused-loss", action="store_true", help="head and cross entropy in one, without the logits")
     a = ap.parse_args()
-    out = train(a.impl, a.steps, a.warmup, a.batch_size, a.depth, a.seed, a.lr, None, a.log, a.fp32, a.graph, a.fused_norm, a.fuse_qkv, a.sdpa)
+    out = train(a.impl, a.steps, a.warmup, a.batch_size, a.depth, a.seed, a.lr, None, a.log, a.fp32, a.graph, a.fused_norm, a.fuse_qkv, a.sdpa,
+                a.rope, a.qk_norm, a.fused_loss)
     if int(os.environ.get("RANK", "0")) == 0:
         out["losses"] = out["losses"][:: max(1, len(out["losses"]) // 20)]
         print(json.dumps(out), flush=True)

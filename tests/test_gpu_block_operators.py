@@ -1,0 +1,134 @@
+"""Rotary positions, query / key norms and the head's loss together, as the image model uses them: values and
+gradients against the same model written out in float64, a training step with every option, and a step
+captured into CUDA graphs."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _fp32_convolution():
+    """torch runs the patch embedding's convolution in TF32 (2^-11) unless told otherwise."""
+    was = torch.backends.cudnn.allow_tf32
+    torch.backends.cudnn.allow_tf32 = False
+    yield
+    torch.backends.cudnn.allow_tf32 = was
+
+
+CFG = dict(img_size=28, patch_size=4, embed_dim=192, num_heads=3, mlp_ratio=4.0)
+
+
+def model64(params, x, rope, qk_norm):
+    """Logits of a depth-1 TinyViT (dropout off) from its float64 parameters."""
+    p = params
+    B, H, dh = x.shape[0], 3, 64
+    x = F.conv2d(x, p["patch_embed.weight"], p["patch_embed.bias"], stride=4).flatten(2).transpose(1, 2)
+    x = torch.cat([p["cls_token"].expand(B, -1, -1), x], 1) + p["pos_embed"]
+    L = x.shape[1]
+    y = F.layer_norm(x, (192,), p["encoder.attn.preln.weight"], p["encoder.attn.preln.bias"])
+    q, k, v = (F.linear(y, p[f"encoder.attn.{n}_proj.weight"], p[f"encoder.attn.{n}_proj.bias"]).view(B, L, H, dh) for n in "qkv")
+    if qk_norm:
+        q, k = ((t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt()) * p[f"encoder.attn.qk_norm.{n}_weight"] for n, t in (("q", q), ("k", k)))
+    if rope:
+        i = torch.arange(49, device=x.device)
+        pos = torch.cat([torch.zeros(1, 2, device=x.device), torch.stack([i // 7 + 1, i % 7 + 1], 1)]).double()
+        f = 100.0 ** (-torch.arange(16, device=x.device).double() / 16)
+        ang = torch.cat([pos[:, :1] * f, pos[:, 1:] * f], 1)[:, None]
+        turn = lambda t: torch.cat([t[..., :32] * ang.cos() - t[..., 32:] * ang.sin(), t[..., :32] * ang.sin() + t[..., 32:] * ang.cos()], -1)  # noqa: E731
+        q, k = turn(q), turn(k)
+    a = torch.softmax(torch.einsum("blhd,bmhd->bhlm", q, k) * math.sqrt(dh), -1)
+    y = torch.einsum("bhlm,bmhd->blhd", a, v).reshape(B, L, 192)
+    x = x + F.linear(y, p["encoder.attn.o_proj.weight"], p["encoder.attn.o_proj.bias"])
+    y = F.layer_norm(x, (192,), p["encoder.ffn.preln.weight"], p["encoder.ffn.preln.bias"])
+    y = F.linear(F.gelu(F.linear(y, p["encoder.ffn.up_proj.weight"], p["encoder.ffn.up_proj.bias"])), p["encoder.ffn.down_proj.weight"],
+                 p["encoder.ffn.down_proj.bias"])
+    return F.linear((x + y)[:, 0], p["mlp_head.weight"], p["mlp_head.bias"])
+
+
+def rel(a, b):
+    return float((a.double() - b).norm() / b.norm().clamp_min(1e-30))
+
+
+@pytest.mark.parametrize("sdpa", [False, True])
+@pytest.mark.parametrize("rope,qk_norm", [(True, False), (False, True), (True, True)])
+def test_model_against_float64(rope, qk_norm, sdpa):
+    """fp32, dropout off.  About a dozen layers in a chain, each off by 2^-20 or less (products over at most 768
+    terms in fp32, the norms' 2^-19 / 2); the softmax carries an error of the scores, |score| <= 8 here, into
+    its weights: 12 * 8 * 2^-20 = 2^-13."""
+    from models import TinyViT
+    torch.manual_seed(0)
+    m = TinyViT(**CFG, linear_impl="torch", rope=rope, qk_norm=qk_norm, sdpa=sdpa).cuda().eval()
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if "qk_norm" in n:
+                p.mul_(1.0 + 0.2 * torch.randn_like(p))
+            elif "_proj.weight" in n:
+                p.mul_(0.5)              # keeps the reference's sqrt(dh)-multiplied scores small without the norm
+    x = torch.rand(16, 1, 28, 28, device="cuda")
+    t = torch.randint(0, 10, (16,), device="cuda")
+    params = {n: p.detach().double().requires_grad_() for n, p in m.named_parameters()}
+    want = model64(params, x.double(), rope, qk_norm)
+    got = m(x)
+    assert rel(got.detach(), want.detach()) <= 2.0 ** -13
+    g64 = torch.autograd.grad(F.cross_entropy(want, t), list(params.values()))
+    g32 = torch.autograd.grad(F.cross_entropy(got, t), list(m.parameters()))
+    for (n, _), a, b in zip(m.named_parameters(), g32, g64):
+        scale = max(float(b.norm()), 1e-6)          # k's bias is close to irrelevant to a softmax: its gradient is a difference of larger terms
+        assert float((a.double() - b).norm()) <= 2.0 ** -12 * scale + 2.0 ** -20, n
+
+
+def test_loss_with_the_head_inside():
+    """model.loss against the loss and gradients of its own bf16 features, in float64 (bounds of one
+    rounding of dl and of the results, 2^-8 each, doubled by the sums' spread)."""
+    from models import TinyViT
+    torch.manual_seed(1)
+    m = TinyViT(**CFG, linear_impl="torch", rope=True, qk_norm=True).cuda().eval()
+    x = torch.rand(64, 1, 28, 28, device="cuda")
+    t = torch.randint(0, 10, (64,), device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = m.loss(x, t)
+        feats = m.features(x)
+    head = (m.mlp_head.weight, m.mlp_head.bias)
+    gw, gb = torch.autograd.grad(loss, head)
+    f64 = feats.detach().to(torch.bfloat16).double()
+    w64 = m.mlp_head.weight.detach().to(torch.bfloat16).double().requires_grad_()
+    b64 = m.mlp_head.bias.detach().double().requires_grad_()
+    want = F.cross_entropy(F.linear(f64, w64, b64), t)
+    hw, hb = torch.autograd.grad(want, (w64, b64))
+    assert gw.dtype == torch.float32 and gb.dtype == torch.float32
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * float(want.detach())
+    assert rel(gw, hw) <= 2.0 ** -15 and rel(gb, hb) <= 1e-5          # 64 tokens: dl in two bf16
+
+
+@pytest.mark.parametrize("impl", ["torch", "cublaslt_nvfp4", "cublaslt_mxfp8"])
+def test_training_step_with_every_option(impl):
+    from backend import ops
+    from models import TinyViT
+    torch.manual_seed(0)
+    m = TinyViT(**CFG, depth=2, linear_impl=impl, fused_norm=True, fuse_qkv=True, rope=True, qk_norm=True).cuda()
+    x = torch.rand(64, 1, 28, 28, device="cuda")
+    t = torch.randint(0, 10, (64,), device="cuda")
+    before = dict(ops.LAUNCHES)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = m.loss(x, t)
+    loss.backward()
+    assert torch.isfinite(loss)
+    for n, p in m.named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all(), n
+    assert ops.LAUNCHES["rotary"] - before["rotary"] == 2 * 3 and ops.LAUNCHES["xent"] > before["xent"]
+    ops.check_status()
+
+
+def test_training_script_replays_the_options_from_graphs():
+    from backend import ops
+    from train_tinyvit import train
+    out = train("cublaslt_nvfp4", steps=3, warmup=1, batch=64, depth=2, seed=0, graph=True, fused_norm=True, fuse_qkv=True, rope=True,
+                qk_norm=True, fused_loss=True)
+    assert all(math.isfinite(v) for v in out["losses"]) and out["rope"] and out["qk_norm"] and out["fused_loss"]
+    eager = train("cublaslt_nvfp4", steps=3, warmup=1, batch=64, depth=2, seed=0, rope=True, qk_norm=True, fused_loss=True)
+    assert all(math.isfinite(v) for v in eager["losses"])
+    ops.check_status()

@@ -84,3 +84,22 @@ def test_argument_errors_of_the_c_entries():
     assert back(heads(), heads(), w, 1e-6, heads(), w, 2, 1, 1, 1, 64, r, buf, 511, None) == -1 and b"workspace" in L.fp4t_last_error()
     assert back(heads(), heads(), w, 1e-6, heads(), w, 2, 1, 1, 1, 64, r, None, 4096, None) == -1 and b"workspace" in L.fp4t_last_error()
     assert back(None, heads(), w, 1e-6, heads(), w, 2, 1, 1, 1, 64, r, buf, 4096, None) == -1
+
+
+def test_model_options_without_a_gpu():
+    """`rope` adds no parameters, `qk_norm` two vectors per block; the plain model's state dict is unchanged."""
+    from models import TinyViT
+    from models.transformer_block import AttentionBlock
+    plain = TinyViT(embed_dim=64, num_heads=4, depth=2)
+    rope = TinyViT(embed_dim=64, num_heads=4, depth=2, rope=True)
+    assert list(plain.state_dict()) == list(rope.state_dict())
+    pos = rope.encoder[0].attn.positions
+    assert pos.shape == (17, 2) and pos[0].tolist() == [0, 0] and pos[1].tolist() == [1, 1] and pos[-1].tolist() == [4, 4]
+    both = TinyViT(embed_dim=64, num_heads=4, depth=2, rope=True, qk_norm=True)
+    extra = set(both.state_dict()) - set(plain.state_dict())
+    assert extra == {f"encoder.{i}.attn.qk_norm.{n}_weight" for i in (0, 1) for n in "qk"}
+    assert both.encoder[0].attn.qk_norm.rotary is not None and both.encoder[0].attn.rotary is None
+    with pytest.raises(ValueError):
+        AttentionBlock(64, 4, rotary=RotaryPositions(16, (8,)))
+    with pytest.raises(NotImplementedError):
+        rope(torch.rand(2, 1, 28, 28))

@@ -18,7 +18,7 @@ DT_BF16, DT_F32 = 0, 1
 SR_NONE, SR_NOISE, SR_HASH = 0, 1, 2
 QOUT_MXFP8, QOUT_NVFP4 = 1, 2
 XENT_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
-STATUS_BAD_TARGET = 41
+STATUS_BAD_TARGET = 60
 
 _c_i64 = ctypes.c_int64
 _c_vp = ctypes.c_void_p
@@ -31,8 +31,7 @@ class Rotary(ctypes.Structure):
                 ("turns", _c_vp), ("axis", _c_vp)]
 
 
-# addresses of one to six fp4t_heads_t in a row (int64 fields: data, heads, stride_batch, stride_token,
-# stride_head), of a Rotary
+# addresses of fp4t_heads_t in a row (int64 fields: data, heads, stride_batch, stride_token, stride_head), of a Rotary
 _p_heads = _p_rotary = _c_vp
 _p_vps = ctypes.POINTER(_c_vp)
 

@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _ext, _lib
 from ._lib import SR_HASH, SR_NOISE, SR_NONE  # noqa: F401  (re-exported)
 
 NVFP4_BLOCK = 16
@@ -21,7 +21,32 @@ import threading
 
 _status = {}
 _tls = threading.local()
-LAUNCHES = {"quantize": 0, "gemm": 0, "misc": 0, "allreduce": 0, "norm": 0, "rotary": 0, "xent": 0}   # kernels enqueued by this process
+
+
+class _Launches(dict):
+    """Kernels enqueued by this process; "rotary" and "xent" are counted where they are launched, in the
+    torch-side module (whose backward passes run without Python)."""
+
+    def _read(self):
+        rotary, xent = _ext.launches()
+        dict.__setitem__(self, "rotary", rotary)
+        dict.__setitem__(self, "xent", xent)
+        return self
+
+    def __getitem__(self, key):
+        return dict.__getitem__(self._read(), key)
+
+    def __iter__(self):          # (also what makes dict(LAUNCHES) go through __getitem__)
+        return dict.__iter__(self._read())
+
+    def values(self):
+        return dict.values(self._read())
+
+    def items(self):
+        return dict.items(self._read())
+
+
+LAUNCHES = _Launches(quantize=0, gemm=0, misc=0, allreduce=0, norm=0, rotary=0, xent=0)
 
 
 def _need_cuda(*tensors):
@@ -530,312 +555,50 @@ def layernorm_backward(dy, x, mean, rstd, gamma):
 
 
 # ------------------------------------------------------------------ rotary positions, query / key norms
-# These calls take a few microseconds of GPU time on a decoding step's tensors, so the host's share is kept
-# small: sizes and strides go over in one array, and nothing is looked up twice.
-_I64 = ctypes.c_int64
-_HEADS = {n: _I64 * (5 * n) for n in range(1, 7)}        # n fp4t_heads_t in a row
-
-
-class _Current(contextlib.AbstractContextManager):
-    """The context of a device that is already current."""
-
-    def __exit__(self, *exc):
-        return None
-
-
-_CURRENT = _Current()
-
-
-def _device_context(index):
-    return _CURRENT if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
-
-
-def _heads(what, tensors, like=None):
-    """Checks one or two [batch, tokens, heads, head_dim] tensors of one dtype, device and shape but for the
-    heads; -> (tensors with unit column stride, the fields of their fp4t_heads_t)."""
-    first = tensors[0] if like is None else like
-    dt, dev, shape = first.dtype, first.device, first.shape
-    if dt is not torch.bfloat16 and dt is not torch.float32:
-        _need_cuda(first)
-        raise ValueError(f"{what} runs on float32 / bfloat16 tensors")
-    out, fields = [], []
-    for t in tensors:
-        if not t.is_cuda:
-            _need_cuda(t)
-        if t.ndim != 4:
-            raise ValueError(f"{what} takes [batch, tokens, heads, head_dim] tensors")
-        if t is not first:
-            if t.dtype is not dt or t.device != dev:
-                raise ValueError(f"{what}: all tensors must have one dtype and one device")
-            sh = t.shape
-            if sh[0] != shape[0] or sh[1] != shape[1] or sh[3] != shape[3]:
-                raise ValueError(f"{what}: tensors must agree in batch, tokens and head_dim")
-        sb, st, hs, unit = t.stride()
-        if unit != 1:
-            t = t.contiguous()
-            sb, st, hs, _ = t.stride()
-        out.append(t)
-        fields += (t.data_ptr(), t.shape[2], sb, st, hs)
-    return out, fields
-
-
-def _outputs(x, fields):
-    """Contiguous results of x's shapes; their fp4t_heads_t fields are appended."""
-    out = []
-    for t in x:
-        y = t.new_empty(t.shape)
-        _, L, H, D = t.shape
-        fields += (y.data_ptr(), H, L * H * D, H * D, D)
-        out.append(y)
-    return out
-
-
-def _rotary_args(what, x, positions, table):
-    """fp4t_rotary_t of a call.  table: (turns int64 [pairs], axis int32 [pairs], axes, interleaved) or None."""
-    if table is None:
-        if positions is not None:
-            raise ValueError(f"{what}: positions without a rotary table")
-        return _lib.Rotary()
-    turns, axis, axes, interleaved = table
-    if positions is None:
-        raise ValueError(f"{what}: a rotary table needs positions")
-    if not (positions.is_cuda and turns.is_cuda and axis.is_cuda):
-        _need_cuda(positions, turns, axis)
-    dt = positions.dtype
-    if dt is not torch.int64 and dt is not torch.int32:
-        raise ValueError(f"{what}: positions must be int32 or int64")
-    dev = x.device
-    if positions.device != dev or turns.device != dev or axis.device != dev:
-        raise ValueError(f"{what}: positions and the rotary table must be on the tensors' device")
-    turned = turns.numel()
-    if turns.dtype is not torch.int64 or axis.dtype is not torch.int32 or turns.ndim != 1 or axis.shape != turns.shape \
-            or not turns.is_contiguous() or not axis.is_contiguous():
-        raise ValueError(f"{what}: the rotary table is an int64 and an int32 vector of one length")
-    batch, tokens, _, dim = x.shape
-    shape, stride = positions.shape, positions.stride()
-    if len(shape) == 1 and axes == 1:
-        shape, stride = (shape[0], 1), (stride[0], 1)
-    if len(shape) not in (2, 3) or shape[-1] != axes or shape[-2] != tokens or (len(shape) == 3 and shape[0] != batch and shape[0] != 1):
-        raise ValueError(f"{what}: positions must be [tokens, {axes}] or [batch, tokens, {axes}], got {tuple(positions.shape)} "
-                         f"for {batch} x {tokens} tokens")
-    if 2 * turned > dim:
-        raise ValueError(f"{what}: {turned} turning pairs do not fit head_dim {dim}")
-    return _lib.Rotary(positions.data_ptr(), int(dt is torch.int64), stride[0] if len(shape) == 3 and shape[0] > 1 else 0, stride[-2],
-                       stride[-1], axes, turned, int(interleaved), turns.data_ptr(), axis.data_ptr())
-
-
-def _head_dim(what, dim):
-    if dim % 2 or not 2 <= dim <= 512:
-        raise ValueError(f"{what} needs an even head_dim of 2 to 512, got {dim}")
-
-
 def rotary(x, positions, table, inverse=False):
     """Rotates one or two [batch, tokens, heads, head_dim] tensors (any strides) by the positions'
     angles (the other way round with inverse=True); -> list of contiguous tensors.
-    positions: int32 / int64 [tokens, axes] or [batch, tokens, axes]; table as in RotaryPositions.table."""
-    x, f = _heads("rotary", x)
-    t = x[0]
-    B, L, _, D = t.shape
-    _head_dim("rotary", D)
-    r = _rotary_args("rotary", t, positions, table)
-    dev, n = t.get_device(), len(x)
-    with _device_context(dev):
-        y = _outputs(x, f)
-        arr = _HEADS[2 * n](*f)
-        at = ctypes.addressof(arr)
-        rc = _lib.lib().fp4t_rotary(at, at + 40 * n, n, t.dtype is torch.float32, B, L, D, ctypes.addressof(r), inverse,
-                                    torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        _lib.check(rc, "fp4t_rotary")
-    LAUNCHES["rotary"] += 1
-    return y
+    positions: int32 / int64 [tokens, axes] or [batch, tokens, axes]; table as in RotaryPositions.table:
+    (turns int64 [pairs], axis int32 [pairs], axes, interleaved)."""
+    return _ext.ext().rotary(list(x), positions, *(table or _NO_TABLE), inverse)
 
 
-def _qk_weights(what, x, weights):
-    out = []
-    for t, w in zip(x, weights):
-        if w.ndim != 1 or w.shape[0] != t.shape[3] or w.device != t.device:
-            raise ValueError(f"{what}: weights must be [head_dim] vectors on the tensors' device")
-        if w.dtype is not torch.float32 or not w.is_contiguous() or w.data_ptr() % 16:
-            w = w.detach().to(torch.float32).contiguous()
-            w = w if w.data_ptr() % 16 == 0 else w.clone()
-        out.append(w)
-    return out
-
-
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+_NO_TABLE = (None, None, 0, False)
 
 
 def qk_norm_rotary_forward(x, weights, eps, positions=None, table=None):
     """RMS norm of every head of one or two [batch, tokens, heads, head_dim] tensors, times its
     tensor's weight [head_dim], then the rotation of `rotary` (none without a table); statistics in fp32."""
-    x, f = _heads("qk_norm_rotary", x)
-    t = x[0]
-    B, L, _, D = t.shape
-    _head_dim("qk_norm_rotary", D)
-    r = _rotary_args("qk_norm_rotary", t, positions, table)
-    dev, n = t.get_device(), len(x)
-    with _device_context(dev):
-        w = _qk_weights("qk_norm_rotary", x, weights)
-        y = _outputs(x, f)
-        arr = _HEADS[2 * n](*f)
-        at = ctypes.addressof(arr)
-        rc = _lib.lib().fp4t_qk_norm_rotary_forward(at, _pointers(w), eps, at + 40 * n, n, t.dtype is torch.float32, B, L, D,
-                                                    ctypes.addressof(r), torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        _lib.check(rc, "fp4t_qk_norm_rotary_forward")
-    LAUNCHES["rotary"] += 1
-    return y
+    return _ext.ext().qk_norm_forward(list(x), list(weights), eps, positions, *(table or _NO_TABLE))
 
 
 def qk_norm_rotary_backward(dy, x, weights, eps, positions=None, table=None):
     """-> (list of dx like x, list of fp32 weight gradients [head_dim]) for the forward above."""
-    x, f = _heads("qk_norm_rotary", x)
-    t = x[0]
-    B, L, _, D = t.shape
-    _head_dim("qk_norm_rotary", D)
-    if any(g.dtype is not t.dtype for g in dy):
-        _need_cuda(*dy)
-        dy = [g.to(t.dtype) for g in dy]
-    dy, fg = _heads("qk_norm_rotary", dy, like=t)
-    if any(g.shape != s.shape for g, s in zip(dy, x)):
-        raise ValueError("dy must have the shapes of x")
-    r = _rotary_args("qk_norm_rotary", t, positions, table)
-    dev, n = t.get_device(), len(x)
-    with _device_context(dev):
-        lib = _lib.lib()
-        w = _qk_weights("qk_norm_rotary", x, weights)
-        dx = _outputs(x, f)
-        arr = _HEADS[3 * n](*f, *fg)
-        at = ctypes.addressof(arr)
-        ws_bytes = lib.fp4t_qk_norm_rotary_backward_workspace_bytes(D)
-        if ws_bytes < 0:
-            raise RuntimeError("fp4t_qk_norm_rotary_backward_workspace_bytes: unsupported shape or device")
-        dw = [torch.empty(D, dtype=torch.float32, device=t.device) for _ in x]
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=t.device)
-        rc = lib.fp4t_qk_norm_rotary_backward(at + 80 * n, at, _pointers(w), eps, at + 40 * n, _pointers(dw), n, t.dtype is torch.float32,
-                                              B, L, D, ctypes.addressof(r), ws.data_ptr(), ws_bytes, torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        _lib.check(rc, "fp4t_qk_norm_rotary_backward")
-    LAUNCHES["rotary"] += 2
-    return dx, dw
+    return _ext.ext().qk_norm_backward(list(dy), list(x), list(weights), eps, positions, *(table or _NO_TABLE))
 
 
 # ------------------------------------------------------------------ linear cross entropy
-def _xent_rows(t, name):
-    """2-D bf16 tensor with rows the kernels can load (unit column stride, 16-byte aligned rows); its pitch."""
-    if not t.is_cuda:
-        _need_cuda(t)
-    if t.ndim != 2 or t.dtype is not torch.bfloat16:
-        raise ValueError(f"linear_cross_entropy: {name} must be a 2-D bfloat16 tensor")
-    rows, dim = t.shape
-    ld, unit = t.stride()
-    if rows <= 1:
-        ld = dim
-    if unit != 1 or ld % 8 or ld < dim or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-        ld = dim
-    return t, ld
+def _reduction(name):
+    try:
+        return _lib.XENT_REDUCTION[name]
+    except KeyError:
+        raise ValueError(f"linear_cross_entropy: unknown reduction {name!r}") from None
 
 
-def _xent_args(h, w, bias, target, reduction):
-    h, ldh = _xent_rows(h, "hidden")
-    w, ldw = _xent_rows(w, "weight")
-    T, D = h.shape
-    V, dim = w.shape
-    if not target.is_cuda:
-        _need_cuda(target)
-    if dim != D:
-        raise ValueError(f"linear_cross_entropy: hidden is {D} wide, weight {dim}")
-    if D % 8 or D == 0:
-        raise ValueError(f"linear_cross_entropy needs a width that is a multiple of 8, got {D}")
-    if V == 0:
-        raise ValueError("linear_cross_entropy: the vocabulary is empty")
-    if target.ndim != 1 or target.shape[0] != T or target.dtype is not torch.int64:
-        raise ValueError(f"linear_cross_entropy: target must be int64 [{T}]")
-    if reduction not in _lib.XENT_REDUCTION:
-        raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
-    dev = h.device
-    if bias is not None:
-        _need_cuda(bias)
-        if bias.ndim != 1 or bias.shape[0] != V or bias.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"linear_cross_entropy: bias must be float32 or bfloat16 [{V}]")
-        if not bias.is_contiguous() or bias.data_ptr() % 16:
-            bias = bias.contiguous()
-            bias = bias if bias.data_ptr() % 16 == 0 else bias.clone()
-    if w.device != dev or target.device != dev or (bias is not None and bias.device != dev):
-        raise ValueError("linear_cross_entropy: all tensors must be on one device")
-    if not target.is_contiguous():
-        target = target.contiguous()
-    return h, ldh, w, ldw, bias, target, T, D, V
-
-
-def _code(dtype):
-    return int(dtype is torch.float32)      # FP4T_DT_BF16 = 0, FP4T_DT_F32 = 1
+def _status_ptr(t):
+    """Address of the status word of a tensor's device (0 for a CPU tensor, which the operator refuses)."""
+    return status_word(t.device).data_ptr() if t.is_cuda else 0
 
 
 def linear_cross_entropy_forward(h, w, bias, target, ignore_index=-100, reduction="mean"):
     """Cross entropy of h @ w.T + bias without the logits.  h [T, D], w [V, D] bf16, bias [V] fp32 / bf16 or
     None, target [T] int64 -> (loss [] or, reduction "none", [T]; lse [T],
     of the counted tokens in order; count []), all fp32."""
-    h, ldh, w, ldw, bias, target, T, D, V = _xent_args(h, w, bias, target, reduction)
-    index, dev = h.get_device(), h.device
-    with _device_context(index):
-        stats = torch.empty(T + 1, dtype=torch.float32, device=dev)
-        lse, count = stats[:T], stats[T]
-        if T == 0:
-            count.zero_()
-            shape = (0,) if reduction == "none" else ()
-            return torch.full(shape, float("nan") if reduction == "mean" else 0.0, device=dev), lse, count
-        loss = torch.empty(T if reduction == "none" else (), dtype=torch.float32, device=dev)
-        L = _lib.lib()
-        ws_bytes = L.fp4t_linear_xent_forward_workspace_bytes(T, D, V)
-        if ws_bytes < 0:
-            _lib.check(-1, "fp4t_linear_xent_forward_workspace_bytes")
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        at = stats.data_ptr()
-        rc = L.fp4t_linear_xent_forward(h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias), 0 if bias is None else _code(bias.dtype),
-                                        target.data_ptr(), T, D, V, ignore_index, _lib.XENT_REDUCTION[reduction], loss.data_ptr(), at,
-                                        at + 4 * T, ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(),
-                                        torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _lib.check(rc, "fp4t_linear_xent_forward")
-    LAUNCHES["xent"] += 1 + 2 * (-(-T // 16384))
-    return loss, lse, count
+    return _ext.ext().xent_forward(h, w, bias, target, ignore_index, _reduction(reduction), _status_ptr(h))
 
 
 def linear_cross_entropy_backward(grad_loss, h, w, bias, target, lse, ignore_index=-100, reduction="mean",
                                   dh_dtype=None, dw_dtype=None, db_dtype=None):
     """-> (dh [T, D], dw [V, D], db [V]) in the dtypes asked for (None: not computed) for the forward above."""
-    h, ldh, w, ldw, bias, target, T, D, V = _xent_args(h, w, bias, target, reduction)
-    if not (grad_loss.is_cuda and lse.is_cuda):
-        _need_cuda(grad_loss, lse)
-    if grad_loss.dtype is not torch.float32 or not grad_loss.is_contiguous():
-        grad_loss = grad_loss.to(torch.float32).contiguous()
-    if grad_loss.numel() != (T if reduction == "none" else 1) or lse.numel() != T or lse.dtype is not torch.float32 or not lse.is_contiguous():
-        raise ValueError("linear_cross_entropy: grad_loss must have the shape of the loss, lse that of the forward's")
-    index, dev = h.get_device(), h.device
-    with _device_context(index):
-        make = torch.empty if T else torch.zeros
-        dh = None if dh_dtype is None else make((T, D), dtype=dh_dtype, device=dev)
-        dw = None if dw_dtype is None else make((V, D), dtype=dw_dtype, device=dev)
-        db = None if db_dtype is None else make((V,), dtype=db_dtype, device=dev)
-        if T == 0 or (dh is None and dw is None and db is None):
-            return dh, dw, db
-        L = _lib.lib()
-        ws_bytes = L.fp4t_linear_xent_backward_workspace_bytes(T, D, V, dh is not None, dw is not None, db is not None)
-        if ws_bytes < 0:
-            raise RuntimeError("fp4t_linear_xent_backward_workspace_bytes: unsupported shape or device")
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        rc = L.fp4t_linear_xent_backward(grad_loss.data_ptr(), h.data_ptr(), ldh, w.data_ptr(), ldw, _lib.ptr(bias),
-                                         0 if bias is None else _code(bias.dtype), target.data_ptr(), lse.data_ptr(), T, D, V, ignore_index,
-                                         _lib.XENT_REDUCTION[reduction], _lib.ptr(dh), _code(dh_dtype), _lib.ptr(dw), _code(dw_dtype),
-                                         _lib.ptr(db), _code(db_dtype), ws.data_ptr(), ws_bytes, status_word(dev).data_ptr(),
-                                         torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _lib.check(rc, "fp4t_linear_xent_backward")
-    LAUNCHES["xent"] += 2 + (dh is not None) + (dw is not None) + (db is not None)
-    return dh, dw, db
+    return _ext.ext().xent_backward(grad_loss, h, w, bias, target, lse, ignore_index, _reduction(reduction), dh_dtype, dw_dtype, db_dtype,
+                                    _status_ptr(h))

@@ -49,7 +49,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // this would overflow there -- a row masked with the type's lowest value, or infinite -- and is
 // subtracted first instead.
 constexpr float kFar = 2e38f;
-constexpr int kXBadTarget = 41;                  // status: a target outside the vocabulary
+constexpr int kXBadTarget = 60;                  // status: a target outside the vocabulary
 
 constexpr int kFew = 64;                         // tokens up to which dl is kept in two bf16 (one K stage)
 constexpr int64_t kTokenBlock = 16384;           // tokens whose partial statistics are held at once
@@ -1336,7 +1336,7 @@ ForwardPlan plan_forward(int64_t tokens, int64_t dim, int64_t vocab) {
   ForwardPlan p;
   p.slots = plan_slots(tokens, dim, false);
   p.block = std::min(tokens, kTokenBlock);
-  p.rows_blocks = tokens <= kRowsTokens && (tokens == 3 ? 4 : tokens) * dim <= kRowsElems ? std::min<int64_t>(ceil_div(vocab, kRowsThreads / 32 * kRowsPerWarp), 148 * 2) : 0;
+  p.rows_blocks = tokens <= kRowsTokens && (tokens == 1 ? 1 : 4) * dim <= kRowsElems ? std::min<int64_t>(ceil_div(vocab, kRowsThreads / 32 * kRowsPerWarp), 148 * 2) : 0;
   p.parts = p.rows_blocks > 0 ? p.rows_blocks : 2 * ceil_div(vocab, width_for(vocab));
   p.lanes = 1;
   while (p.lanes < 8 && p.lanes < tokens) p.lanes <<= 1;
@@ -1462,8 +1462,8 @@ extern "C" int fp4t_linear_xent_forward(const void* h, int64_t ldh, const void* 
       r.target = sl.target;
       r.part = g.part;
       r.picked = g.picked;
-      auto kern = tokens == 1 ? xent_rows_kernel<1> : tokens == 2 ? xent_rows_kernel<2> : xent_rows_kernel<4>;
-      rc = launch_small_shared(kern, (int)p.rows_blocks, kRowsThreads, (tokens <= 2 ? tokens : 4) * dim * 2, s, r);
+      auto kern = tokens == 1 ? xent_rows_kernel<1> : xent_rows_kernel<4>;
+      rc = launch_small_shared(kern, (int)p.rows_blocks, kRowsThreads, (tokens == 1 ? 1 : 4) * dim * 2, s, r);
     } else
       rc = launch_xent<kStats>(width_for(vocab), Operand{static_cast<const __nv_bfloat16*>(h) + t0 * ldh, rows, dim, ldh}, Operand{w, vocab, dim, ldw},
                              Operand{sl.packed + t0 * dim, rows, dim, dim}, nullptr, 0, g, dim, s);

@@ -12,45 +12,10 @@ rounded to bf16, as F.linear does there; their gradients come back in fp32, stra
 accumulators."""
 from __future__ import annotations
 
-import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from backend import ops as _ops
-
-
-def _operand(t, name):
-    if t.dtype == torch.bfloat16:
-        return t
-    if t.dtype == torch.float32 and torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
-        return t.to(torch.bfloat16)
-    raise ValueError(f"linear_cross_entropy: {name} is {t.dtype}; it takes bfloat16 (float32 too under bfloat16 autocast)")
-
-
-def _forward(hidden, weight, bias, target, ignore_index, reduction):
-    h, w, t = _operand(hidden, "hidden"), _operand(weight, "weight"), target
-    if hidden.ndim != 2:
-        h, t = h.reshape(-1, hidden.shape[-1]), target.reshape(-1)
-    loss, lse, _ = _ops.linear_cross_entropy_forward(h, w, bias, t, ignore_index, reduction)
-    return h, w, t, loss.view(target.shape) if reduction == "none" else loss, lse
-
-
-class _LinearCrossEntropyFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, target, ignore_index, reduction):
-        ctx.dtypes = hidden.dtype, weight.dtype, None if bias is None else bias.dtype
-        ctx.shape, ctx.args = hidden.shape, (ignore_index, reduction)
-        h, w, t, loss, lse = _forward(hidden, weight, bias, target, ignore_index, reduction)
-        ctx.save_for_backward(h, w, bias, t, lse)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        h, w, bias, t, lse = ctx.saved_tensors
-        want = [dt if need else None for dt, need in zip(ctx.dtypes, ctx.needs_input_grad)]
-        dh, dw, db = _ops.linear_cross_entropy_backward(grad.reshape(-1), h, w, bias, t, lse, *ctx.args, *want)
-        return None if dh is None else dh.view(ctx.shape), dw, db, None, None, None     # (a head frozen in training: only dh)
+from backend._ext import ext as _ext
 
 
 def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, reduction="mean"):
@@ -59,12 +24,7 @@ def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, r
     hidden [..., D], weight [V, D] (D a multiple of 8), bias [V] (float32 or bfloat16), target [...] int64.
     reduction "mean" (over the tokens whose target is not ignore_index), "sum" or "none"; the result is fp32.
     A target outside the vocabulary makes its loss NaN and is reported by backend.ops.check_status()."""
-    if hidden.ndim < 1 or weight.ndim != 2 or target.shape != hidden.shape[:-1]:
-        raise ValueError("linear_cross_entropy takes hidden [..., D], weight [V, D] and target [...], got "
-                         f"{tuple(hidden.shape)}, {tuple(weight.shape)} and {tuple(target.shape)}")
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        return _LinearCrossEntropyFn.apply(hidden, weight, bias, target, int(ignore_index), reduction)
-    return _forward(hidden, weight, bias, target, int(ignore_index), reduction)[3]
+    return _ext().xent_call(hidden, weight, bias, target, ignore_index, _ops._reduction(reduction), _ops._status_ptr(hidden))
 
 
 class LinearCrossEntropy(nn.Module):

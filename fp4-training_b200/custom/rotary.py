@@ -15,55 +15,11 @@ import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
-from backend import ops as _ops
-
-
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, positions, table, *x):
-        ctx.table = table[2:]
-        ctx.save_for_backward(positions, table[0], table[1])
-        return tuple(_ops.rotary(x, positions, table))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *dy):
-        positions, turns, axis = ctx.saved_tensors
-        dx = _ops.rotary(dy, positions, (turns, axis) + ctx.table, inverse=True)     # a rotation's transpose
-        return (None, None, *dx)
+from backend._ext import ext as _ext
 
 
-class _QKNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, positions, table, eps, count, *args):
-        x, w = args[:count], args[count:]
-        ctx.eps, ctx.count = eps, count
-        ctx.table = None if table is None else table[2:]
-        ctx.save_for_backward(positions, *(table[:2] if table is not None else (None, None)), *args)
-        return tuple(_ops.qk_norm_rotary_forward(x, w, eps, positions, table))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *dy):
-        positions, turns, axis, *args = ctx.saved_tensors
-        x, w = args[:ctx.count], args[ctx.count:]
-        table = None if ctx.table is None else (turns, axis) + ctx.table
-        dx, dw = _ops.qk_norm_rotary_backward(dy, x, w, ctx.eps, positions, table)
-        return (None, None, None, None, *dx, *[g if t.dtype is torch.float32 else g.to(t.dtype) for g, t in zip(dw, w)])
-
-
-def _rotate(positions, table, *x):
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in x)):
-        return _ops.rotary(x, positions, table)
-    return _RotaryFn.apply(positions, table, *x)
-
-
-def _qk_norm(positions, table, eps, q, k, wq, wk):
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or wq.requires_grad or wk.requires_grad)):
-        return _ops.qk_norm_rotary_forward((q, k), (wq, wk), eps, positions, table)
-    return _QKNormFn.apply(positions, table, eps, 2, q, k, wq, wk)
+_NO_TABLE = (None, None, 0, False)
 
 
 class RotaryPositions(nn.Module):
@@ -123,18 +79,15 @@ class RotaryPositions(nn.Module):
         return buffers["turns"], buffers["axis"], len(self.sections), self.layout == "interleaved"
 
     def _check(self, x):
-        if x[0].shape[-1] != self.head_dim:
-            raise ValueError(f"head_dim {x[0].shape[-1]} is not this module's {self.head_dim}")
+        if x.shape[-1] != self.head_dim:
+            raise ValueError(f"head_dim {x.shape[-1]} is not this module's {self.head_dim}")
 
     def forward(self, *x, positions):
         """rotary(q, k, positions=p) -> (q', k'), or rotary(x, positions=p) -> x'."""
         if len(x) not in (1, 2):
             raise ValueError("RotaryPositions takes one or two tensors")
-        self._check(x)
-        if x[0].ndim == 3:
-            y = [o.squeeze(0) for o in _rotate(positions, self.table, *[t.unsqueeze(0) for t in x])]
-        else:
-            y = _rotate(positions, self.table, *x)
+        self._check(x[0])
+        y = _ext().rotary_call(x[0], x[1] if len(x) == 2 else None, positions, *self.table)
         return tuple(y) if len(x) == 2 else y[0]
 
     def extra_repr(self):
@@ -161,11 +114,9 @@ class FusedQKNorm(nn.Module):
     def forward(self, q, k, positions=None):
         if q.shape[-1] != self.head_dim:
             raise ValueError(f"head_dim {q.shape[-1]} is not this module's {self.head_dim}")
-        table = None if self.rotary is None else self.rotary.table
-        if q.ndim == 3:
-            qo, ko = _qk_norm(positions, table, self.eps, q.unsqueeze(0), k.unsqueeze(0), self.q_weight, self.k_weight)
-            return qo.squeeze(0), ko.squeeze(0)
-        return tuple(_qk_norm(positions, table, self.eps, q, k, self.q_weight, self.k_weight))
+        table = _NO_TABLE if self.rotary is None else self.rotary.table
+        params = self._parameters
+        return tuple(_ext().qk_norm_call(q, k, params["q_weight"], params["k_weight"], positions, *table, self.eps))
 
     def extra_repr(self):
         return f"head_dim={self.head_dim}, eps={self.eps}"

@@ -531,7 +531,7 @@ FP4T_API int fp4t_qk_norm_rotary_backward(const fp4t_heads_t* dy, const fp4t_hea
  * h [tokens, dim] and w [vocab, dim]: bf16 rows, pitches ldh / ldw in elements (multiples of 8), dim % 8 == 0;
  * bias [vocab] f32 or bf16, or null; target [tokens] int64.  Tokens whose target is ignore_index have loss
  * 0, count for nothing in the mean and get zero gradients.  A target outside [0, vocab) that is not
- * ignore_index makes its token's loss NaN and leaves 41 in the status word.  With FP4T_XENT_MEAN and no
+ * ignore_index makes its token's loss NaN and leaves 60 in the status word.  With FP4T_XENT_MEAN and no
  * counted token the loss is NaN (0 / 0) and the gradients are zero.  Ignored tokens cost no products (the
  * counted ones are packed together on the device) and nothing of their rows of h reaches a result.  Pointers are 16-byte aligned,
  * tokens >= 1.  Losses, lse and sums in fp32 (the mean's sum in fp64); logits are accumulated in fp32.

@@ -132,3 +132,72 @@ def test_training_script_replays_the_options_from_graphs():
     eager = train("cublaslt_nvfp4", steps=3, warmup=1, batch=64, depth=2, seed=0, rope=True, qk_norm=True, fused_loss=True)
     assert all(math.isfinite(v) for v in eager["losses"])
     ops.check_status()
+
+
+def test_each_operator_differentiates_once():
+    """A gradient taken with create_graph is there; asking for the gradient's gradient raises."""
+    from custom import FusedQKNorm, RotaryPositions, linear_cross_entropy
+    rot = RotaryPositions(64, (32,)).cuda()
+    norm = FusedQKNorm(64, rotary=rot).cuda()
+    p = torch.arange(5, device="cuda")
+    q = torch.randn(1, 5, 2, 64, device="cuda", requires_grad=True)
+    h = torch.randn(8, 64, device="cuda").bfloat16().requires_grad_()
+    w = torch.randn(30, 64, device="cuda").bfloat16().requires_grad_()
+    t = torch.arange(8, device="cuda")
+    for f, leaf in ((lambda: rot(q, positions=p).square().sum(), q), (lambda: norm(q, q, p)[0].square().sum(), q),
+                    (lambda: linear_cross_entropy(h, w, t).square(), h)):
+        (plain,) = torch.autograd.grad(f(), leaf)
+        (g,) = torch.autograd.grad(f(), leaf, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="differentiates once"):
+            torch.autograd.grad(g.float().square().sum(), leaf)
+
+
+def test_partial_gradients_and_unused_outputs():
+    """Only some inputs need gradients; only one of two outputs is used."""
+    from custom import FusedQKNorm, RotaryPositions, linear_cross_entropy
+    rot = RotaryPositions(64, (32,)).cuda()
+    norm = FusedQKNorm(64, rotary=rot).cuda()
+    p = torch.arange(5, device="cuda")
+    q = torch.randn(1, 5, 2, 64, device="cuda", requires_grad=True)
+    k = torch.randn(1, 5, 1, 64, device="cuda")
+    a, b = rot(q, k, positions=p)
+    assert a.requires_grad
+    (g,) = torch.autograd.grad(a.sum(), q)
+    assert torch.equal(g, torch.autograd.grad(rot(q, positions=p).sum(), q)[0])
+    k.requires_grad_()
+    a, b = norm(q, k, p)
+    gq, gk, gw = torch.autograd.grad(b.sum(), [q, k, norm.q_weight])
+    assert (gq == 0).all() and (gw == 0).all() and (gk != 0).any()
+    h = torch.randn(70, 64, device="cuda").bfloat16().requires_grad_()
+    w = torch.randn(30, 64, device="cuda").bfloat16()
+    t = torch.arange(70, device="cuda") % 30
+    (gh,) = torch.autograd.grad(linear_cross_entropy(h, w, t), h)          # a frozen head
+    w2 = w.clone().requires_grad_()
+    both = torch.autograd.grad(linear_cross_entropy(h, w2, t), [h, w2])
+    assert torch.equal(gh, both[0])
+    (gw,) = torch.autograd.grad(linear_cross_entropy(h.detach(), w2, t), w2)
+    assert torch.equal(gw, both[1])
+    with torch.no_grad():
+        assert not linear_cross_entropy(h, w2, t).requires_grad
+
+
+def test_weights_of_other_dtypes():
+    """bf16 parameters: computed in fp32, gradients in their dtype."""
+    from custom import FusedQKNorm
+    norm = FusedQKNorm(64).cuda().bfloat16()
+    q = torch.randn(2, 9, 2, 64, device="cuda", requires_grad=True)
+    a, b = norm(q, q)
+    g = torch.autograd.grad(a.sum() + b.square().sum(), [q, norm.q_weight, norm.k_weight])
+    assert g[1].dtype == torch.bfloat16 and g[0].dtype == torch.float32 and all(torch.isfinite(x).all() for x in g)
+
+
+def test_parameters_accumulate_like_any_others():
+    from custom import FusedQKNorm
+    norm = FusedQKNorm(64).cuda()
+    q = torch.randn(2, 9, 2, 64, device="cuda")
+    for _ in range(2):
+        a, b = norm(q, q)
+        (a.square().sum() + b.sum()).backward()
+    once = torch.autograd.grad((lambda o: o[0].square().sum() + o[1].sum())(norm(q, q)), [norm.q_weight, norm.k_weight])
+    assert torch.allclose(norm.q_weight.grad, 2 * once[0]) and torch.allclose(norm.k_weight.grad, 2 * once[1])

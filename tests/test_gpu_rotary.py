@@ -263,14 +263,15 @@ def test_empty_and_broadcast():
 def test_in_place_through_the_c_entry():
     import ctypes
 
-    from backend import _lib, ops
+    from backend import _lib
     from custom import RotaryPositions
     rot = RotaryPositions(64, (16, 16)).cuda()
     x = torch.randn(2, 30, 3, 64, device="cuda")
     p = torch.randint(0, 99, (30, 2), device="cuda")
     want = rot(x, positions=p)
     arr = (ctypes.c_int64 * 5)(x.data_ptr(), 3, 30 * 3 * 64, 3 * 64, 64)
-    r = ops._rotary_args("rotary", x, p, rot.table)
+    turns, axis, axes, interleaved = rot.table
+    r = _lib.Rotary(p.data_ptr(), 1, 0, p.stride(0), p.stride(1), axes, turns.numel(), int(interleaved), turns.data_ptr(), axis.data_ptr())
     _lib.check(_lib.lib().fp4t_rotary(arr, arr, 1, _lib.DT_F32, 2, 30, 64, ctypes.byref(r), 0, _lib.stream_ptr(x.device)), "fp4t_rotary")
     assert torch.equal(x, want)
 

@@ -10,6 +10,9 @@
 // wraps modulo one turn by itself, so a position of a million is as exact as one of ten (an fp32
 // product is off by 0.06 radians there) and costs one integer multiply, no fp64.
 //
+// The arithmetic is packed, two floats an instruction: element by element the norm kernels took 211
+// instructions per lane and head and were bound by their issue.
+//
 // A head is held by a group of 1 to 32 lanes, up to eight pairs (two 16-byte vectors of bf16) a lane, so the
 // norm is a shuffle reduction inside the group and every element is read and written once:
 // HBM-bound (forward 4 bytes per bf16 element, norm backward 6).  A group walks heads of ONE token,
@@ -19,6 +22,7 @@
 #include <algorithm>
 
 #include "fp4t_common.cuh"
+#include "fp4t_pack.cuh"
 
 namespace fp4t {
 namespace {
@@ -159,48 +163,6 @@ __device__ __forceinline__ void chunk_offsets(int p0, int turned, int& ea, int& 
 }
 
 enum { kRotate = 0, kNormRotate = 1, kNormRotateBackward = 2 };
-
-// Two floats in one 64-bit register pair, worked on by one instruction (the norm kernels are bound by
-// instruction issue otherwise: 211 per lane and head without, see below); one float where chunks are single pairs.
-template <int W>
-struct Pack {
-  uint64_t v;
-  static __device__ __forceinline__ Pack of(const float* p) {
-    Pack r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(p[0]), "f"(p[1]));
-    return r;
-  }
-  static __device__ __forceinline__ Pack all(float x) {
-    const float t[2] = {x, x};
-    return of(t);
-  }
-  __device__ __forceinline__ void to(float* p) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(p[0]), "=f"(p[1]) : "l"(v)); }
-  __device__ __forceinline__ float sum() const {
-    float t[2];
-    to(t);
-    return t[0] + t[1];
-  }
-};
-template <>
-struct Pack<1> {
-  float v;
-  static __device__ __forceinline__ Pack of(const float* p) { return Pack{p[0]}; }
-  static __device__ __forceinline__ Pack all(float x) { return Pack{x}; }
-  __device__ __forceinline__ void to(float* p) const { p[0] = v; }
-  __device__ __forceinline__ float sum() const { return v; }
-};
-__device__ __forceinline__ Pack<2> mul(Pack<2> a, Pack<2> b) {
-  Pack<2> r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pack<2> fma(Pack<2> a, Pack<2> b, Pack<2> c) {
-  Pack<2> r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Pack<1> mul(Pack<1> a, Pack<1> b) { return Pack<1>{a.v * b.v}; }
-__device__ __forceinline__ Pack<1> fma(Pack<1> a, Pack<1> b, Pack<1> c) { return Pack<1>{fmaf(a.v, b.v, c.v)}; }
 
 // What a lane holds of a head: kSlots chunks of V pairs each (V * kSlots = 8 pairs), chunk s of lane j
 // starting at pair (j + s * group) * V.

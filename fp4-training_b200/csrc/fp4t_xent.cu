@@ -33,6 +33,7 @@
 #include <algorithm>
 
 #include "fp4t_common.cuh"
+#include "fp4t_pack.cuh"
 #include "fp4t_tcgen05.cuh"
 
 namespace fp4t {
@@ -88,12 +89,16 @@ struct XParams {
   int32_t* status;
 };
 
-template <int kBN>
+// kStats stores nothing through shared memory and gets a seventh stage instead; the others stage four bf16
+// (two fp32) chunks per epilogue warp, so that a chunk does not wait for the copy engine to have read the one
+// before the last (with two bf16 chunks a tile's epilogue took 4600 cycles, more than eight K stages' products).
+template <int kMode, int kBN>
 struct XCfg {
   static constexpr int kBRows = kBN / 2;                         // rows of the second operand per CTA
   static constexpr int kABytes = 128 * kXK * 2, kBBytes = kBRows * kXK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kEpiBytes = kXEpiWarps * 4096;
+  static constexpr int kEpiWarpBytes = kMode == kStats ? 0 : 8192;
+  static constexpr int kEpiBytes = kXEpiWarps * kEpiWarpBytes;
   static constexpr int kBarBytes = 512;
   static constexpr int kBudget = 227 * 1024 - kEpiBytes - kBarBytes;
   static constexpr int kStages = kBudget / kStageBytes > 8 ? 8 : kBudget / kStageBytes;
@@ -221,11 +226,11 @@ __device__ __forceinline__ float column_sums(const float (&v)[32], int lane) {
 }
 
 // One 32 x 32 chunk (a row per lane) to a swizzled staging tile and from there with one tiled TMA
-// store, clipped at the matrix edges.  bf16: two 2-KB tiles that alternate; fp32: one of 4 KB.
+// store, clipped at the matrix edges.  `buf`: the warp's 8 KB, four 2-KB tiles of bf16 or two of fp32 in turn.
 __device__ __forceinline__ void store_chunk_bf16(const CUtensorMap* map, uint8_t* buf, uint32_t& n_emit, int lane, int row, int col,
                                                  const float (&v)[32]) {
-  uint8_t* tile = buf + (n_emit & 1u) * 2048;
-  if (lane == 0) bulk_wait_read<1>();
+  uint8_t* tile = buf + (n_emit & 3u) * 2048;
+  if (lane == 0) bulk_wait_read<3>();
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -245,18 +250,40 @@ __device__ __forceinline__ void store_chunk_bf16(const CUtensorMap* map, uint8_t
   }
   ++n_emit;
 }
-__device__ __forceinline__ void store_chunk_f32(const CUtensorMap* map, uint8_t* buf, int lane, int row, int col, const float (&v)[32]) {
-  if (lane == 0) bulk_wait_read<0>();
+__device__ __forceinline__ void store_chunk_f32(const CUtensorMap* map, uint8_t* buf, uint32_t& n_emit, int lane, int row, int col,
+                                                const float (&v)[32]) {
+  uint8_t* tile = buf + (n_emit & 1u) * 4096;
+  if (lane == 0) bulk_wait_read<1>();
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    *reinterpret_cast<float4*>(tile + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   fence_async_smem();
   __syncwarp();
   if (lane == 0) {
-    tma_store_2d(map, smem_u32(buf), col, row);
+    tma_store_2d(map, smem_u32(tile), col, row);
     bulk_commit();
   }
+  ++n_emit;
+}
+
+// The wait for a tcgen05.ld that was issued before other work: its registers pass through, so that nothing
+// reads them earlier.
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// v <- v log2(e) - ref, two at a time
+__device__ __forceinline__ void scale_to_log2(float (&v)[32], float ref) {
+  const Pack<2> l = Pack<2>::all(kLog2e), m = Pack<2>::all(-ref);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) fma(Pack<2>::of(v + j), l, m).to(v + j);
 }
 
 // The same chunk to rows that are not neighbours: each lane its own (columns are a multiple of 8).
@@ -286,7 +313,7 @@ template <int kMode, int kBN>
 __global__ void __launch_bounds__(kXThreads, 1)
 xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_packed, const __grid_constant__ CUtensorMap map_d, const XParams gp) {
-  using C = XCfg<kBN>;
+  using C = XCfg<kMode, kBN>;
   XParams g = gp;
   constexpr bool kAMn = kMode == kProductT, kBMn = kMode == kProduct || kMode == kProductT;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -442,7 +469,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   } else if (warp >= 4) {
     // ------------------------------ epilogue (each CTA) ------------------------------
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    uint8_t* buf = smem + C::kEpi0 + (warp - 4) * 4096;
+    uint8_t* buf = smem + C::kEpi0 + (warp - 4) * C::kEpiWarpBytes;
     uint32_t n_emit = 0;
     // a scalar gradient of the loss scales the products (and db), one per token is part of dl
     float scale = 1.f;
@@ -478,17 +505,20 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           lse = row_ok ? __ldg(g.lse + slot) : 0.f;
           gr = g.grad_per_row ? (row_ok ? __ldg(g.grad + __ldg(g.token + slot)) : 0.f) : 1.f;
         }
-#pragma unroll 1
-        for (int c = 0; c < C::kHalf / 32; ++c) {
-          uint32_t r[32];
-          tc_ld32(acc + (uint32_t)(c * 32), r);
-          tc_wait_ld();
-          if (c == C::kHalf / 32 - 1) release();
+        const bool all_ok = __all_sync(0xFFFFFFFFu, row_ok);
+        constexpr int kN = C::kHalf / 32;
+        uint32_t r[2][32];
+        tc_ld32(acc, r[0]);
+#pragma unroll
+        for (int c = 0; c < kN; ++c) {
+          tc_wait_ld(r[c & 1]);
+          if (c + 1 < kN) tc_ld32(acc + (uint32_t)((c + 1) * 32), r[(c + 1) & 1]);    // under this chunk's work
+          else release();
           const int col = colbase + c * 32;
           if (col >= g.cols || row0 >= row_end) continue;     // warp-uniform
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[c & 1][j]);
           add_bias(g, col, v);
           if (kMode == kStats) {
             if (col + 32 > g.cols) {
@@ -501,22 +531,23 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
               for (int j = 0; j < 32; ++j)
                 if (mine == c * 32 + j) x_y = v[j];
             }
-            float top = v[0];
+            float top[8];
 #pragma unroll
-            for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
-            const float mn = fmaxf(m, top);
+            for (int j = 0; j < 8; ++j) top[j] = fmaxf(fmaxf(v[j], v[j + 8]), fmaxf(v[j + 16], v[j + 24]));
+            const float mn = fmaxf(fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))),
+                                   fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
             if (fabsf(mn) < kFar) {              // by row: its result does not depend on its neighbours
               const float ref = mn * kLog2e;
-              float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+              scale_to_log2(v, ref);
+              Pack<2> sum[4];
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                s0 += exp2_fast(fmaf(v[j], kLog2e, -ref));
-                s1 += exp2_fast(fmaf(v[j + 1], kLog2e, -ref));
-                s2 += exp2_fast(fmaf(v[j + 2], kLog2e, -ref));
-                s3 += exp2_fast(fmaf(v[j + 3], kLog2e, -ref));
+              for (int j = 0; j < 32; j += 2) {
+                const float e[2] = {exp2_fast(v[j]), exp2_fast(v[j + 1])};
+                sum[(j >> 1) & 3] = j < 8 ? Pack<2>::of(e) : add(sum[(j >> 1) & 3], Pack<2>::of(e));
               }
               // ref is mn log2(e) rounded, the same error in all terms: the residual takes it out of their sum
-              s = fmaf(s, exp2_fast((m - mn) * kLog2e), ((s0 + s1) + (s2 + s3)) * fmaf(fmaf(mn, kLog2e, -ref), -kLn2, 1.f));
+              s = fmaf(s, exp2_fast((m - mn) * kLog2e),
+                       add(add(sum[0], sum[1]), add(sum[2], sum[3])).sum() * fmaf(fmaf(mn, kLog2e, -ref), -kLn2, 1.f));
             } else {
               const float ref = mn == -INFINITY ? 0.f : mn;           // a row of -inf so far: all terms are 0
               float s0 = 0.f;
@@ -527,9 +558,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             m = mn;
           } else {
             if (fabsf(lse) < kFar) {
-              const float lse2 = lse * kLog2e;
+              scale_to_log2(v, lse * kLog2e);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -lse2));
+              for (int j = 0; j < 32; ++j) v[j] = exp2_fast(v[j]);
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = exp2_fast((v[j] - lse) * kLog2e);
@@ -539,8 +570,14 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
               for (int j = 0; j < 32; ++j)
                 if (mine == c * 32 + j) v[j] -= 1.f;
             }
+            if (g.grad_per_row) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = row_ok ? v[j] * gr : 0.f;
+              for (int j = 0; j < 32; ++j) v[j] *= gr;
+            }
+            if (!all_ok) {                                    // rows without a token: zeros, whatever the tile holds there
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = row_ok ? v[j] : 0.f;
+            }
             if (g.col_part != nullptr && (!g.few || row0 < kFew)) {
               const float sum = column_sums(v, lane) * scale;
               if (col + lane < g.cols) g.col_part[(int64_t)(row0 >> 5) * g.col_ld + col + lane] = sum;
@@ -561,17 +598,19 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         void* out_row = nullptr;
         if (kMode == kProduct && g.out != nullptr && !dense && row_ok)
           out_row = static_cast<uint8_t*>(g.out) + (int64_t)__ldg(g.token + row) * g.cols * (g.out_f32 ? 4 : 2);
-#pragma unroll 1
-        for (int c = 0; c < C::kHalf / 32; ++c) {
-          uint32_t r[32];
-          tc_ld32(acc + (uint32_t)(c * 32), r);
-          tc_wait_ld();
-          if (c == C::kHalf / 32 - 1) release();
+        constexpr int kN = C::kHalf / 32;
+        uint32_t r[2][32];
+        tc_ld32(acc, r[0]);
+#pragma unroll
+        for (int c = 0; c < kN; ++c) {
+          tc_wait_ld(r[c & 1]);
+          if (c + 1 < kN) tc_ld32(acc + (uint32_t)((c + 1) * 32), r[(c + 1) & 1]);
+          else release();
           const int col = colbase + c * 32;
           if (col >= g.cols || row0 >= g.rows) continue;
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = nothing ? 0.f : __uint_as_float(r[j]) * scale;
+          for (int j = 0; j < 32; ++j) v[j] = nothing ? 0.f : __uint_as_float(r[c & 1][j]) * scale;
           if (g.acc != nullptr && row_ok && !sliced) {         // columns are a multiple of 8: whole vectors
             const float4* p = reinterpret_cast<const float4*>(g.acc + (int64_t)row * g.ldacc + col);
 #pragma unroll
@@ -583,9 +622,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
           }
           const int srow = row0 + t.split * g.slice_rows;
-          if (sliced) store_chunk_f32(&map_packed, buf, lane, srow, col, v);
+          if (sliced) store_chunk_f32(&map_packed, buf, n_emit, lane, srow, col, v);
           else if (kMode == kProduct && g.out != nullptr && !dense) store_row_chunk(out_row, g.out_f32, col, g.cols, v);
-          else if (g.out_f32) store_chunk_f32(&map_d, buf, lane, srow, col, v);
+          else if (g.out_f32) store_chunk_f32(&map_d, buf, n_emit, lane, srow, col, v);
           else store_chunk_bf16(&map_d, buf, n_emit, lane, srow, col, v);
         }
       }
@@ -703,29 +742,32 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
     }
     __syncthreads();
     if (!dense) {
-      for (int i = warp; i < total; i += kPackThreads / 32) {
-        const uint4* from = reinterpret_cast<const uint4*>(p.h + (int64_t)source[i] * p.ldh);
-        uint4* to = reinterpret_cast<uint4*>(p.packed + (int64_t)(before + i) * p.dim);
-        for (int c0 = lane; c0 < p.dim / 8; c0 += 128) {
-          uint4 v[4];
+      const int vecs = p.dim / 8;
+      for (int64_t c0 = threadIdx.x; c0 < (int64_t)total * vecs; c0 += 4 * kPackThreads) {
+        uint4 v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (c0 + 32 * k < p.dim / 8) v[k] = __ldg(from + c0 + 32 * k);
+        for (int k = 0; k < 4; ++k) {
+          const int64_t c = c0 + k * kPackThreads;
+          const int i = (int)(c / vecs);
+          if (i < total) v[k] = __ldg(reinterpret_cast<const uint4*>(p.h + (int64_t)source[i] * p.ldh) + (c - (int64_t)i * vecs));
+        }
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (c0 + 32 * k < p.dim / 8) {
-              to[c0 + 32 * k] = v[k];
-              if (p.few) to[c0 + 32 * k + (int64_t)kFew * (p.dim / 8)] = v[k];
-            }
+        for (int k = 0; k < 4; ++k) {
+          const int64_t c = c0 + k * kPackThreads;
+          if (c < (int64_t)total * vecs) {
+            uint4* to = reinterpret_cast<uint4*>(p.packed) + (int64_t)before * vecs + c;
+            to[0] = v[k];
+            if (p.few) to[(int64_t)kFew * vecs] = v[k];
+          }
         }
       }
       if (p.dh != nullptr) {
-        const int vecs = p.dim / (p.dh_f32 ? 4 : 8);
+        const int dvecs = p.dim / (p.dh_f32 ? 4 : 8);
         for (int i = 0; i < 32; ++i) {            // a warp its own 32 tokens
           const int tt = base + warp * 32 + i;
           if (tt < t1 && !((votes >> i) & 1u)) {
-            uint4* to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.dh) + (int64_t)tt * vecs * 16);
-            for (int c = lane; c < vecs; c += 32) to[c] = make_uint4(0u, 0u, 0u, 0u);
+            uint4* to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.dh) + (int64_t)tt * dvecs * 16);
+            for (int c = lane; c < dvecs; c += 32) to[c] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
       }
@@ -733,9 +775,10 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
     before += total;
   }
   // the rows behind the last slot that the last K stage of dW reads are zero
-  if (!dense && blockIdx.x == gridDim.x - 1) {
+  if (!dense) {
     const int end = p.few ? kFew : min(p.tokens, (all + kXK - 1) / kXK * kXK);
-    for (int64_t c = (int64_t)all * (p.dim / 8) + threadIdx.x; c < (int64_t)end * (p.dim / 8); c += kPackThreads) {
+    for (int64_t c = (int64_t)all * (p.dim / 8) + blockIdx.x * kPackThreads + threadIdx.x; c < (int64_t)end * (p.dim / 8);
+         c += (int64_t)gridDim.x * kPackThreads) {
       reinterpret_cast<uint4*>(p.packed)[c] = make_uint4(0u, 0u, 0u, 0u);
       if (p.few) reinterpret_cast<uint4*>(p.packed)[c + (int64_t)kFew * (p.dim / 8)] = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -1049,11 +1092,11 @@ int xent_clusters() {
   if (cached[dev] == 0) {
     auto kern = xent_gemm_kernel<kMode, kBN>;
     int n = -1;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, XCfg<kBN>::kSmemBytes) == cudaSuccess) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, XCfg<kMode, kBN>::kSmemBytes) == cudaSuccess) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(2 * 148, 1, 1);
       cfg.blockDim = dim3(kXThreads, 1, 1);
-      cfg.dynamicSmemBytes = XCfg<kBN>::kSmemBytes;
+      cfg.dynamicSmemBytes = XCfg<kMode, kBN>::kSmemBytes;
       cudaLaunchAttribute attr;
       attr.id = cudaLaunchAttributeClusterDimension;
       attr.val.clusterDim.x = 2;
@@ -1114,7 +1157,7 @@ int bf16_map(CUtensorMap* map, const Operand& o, int box_inner, int box_outer, C
 // kProduct the fp32 slices.
 template <int kMode, int kBN>
 int launch_width(const Operand& a, const Operand& b, const Operand& packed, void* out, int64_t ldo, XParams g, int64_t k, cudaStream_t stream) {
-  using C = XCfg<kBN>;
+  using C = XCfg<kMode, kBN>;
   constexpr bool kAMn = kMode == kProductT, kBMn = kMode == kProduct || kMode == kProductT;
   const int resident = xent_clusters<kMode, kBN>();
   int clusters = cluster_budget();
@@ -1281,7 +1324,7 @@ struct SlotPlan {
 };
 SlotPlan plan_slots(int64_t tokens, int64_t dim, bool backward) {
   SlotPlan p;
-  p.run = round_up(ceil_div(tokens, 148 * 4), 8);        // a warp copies a row at a time, a block has eight
+  p.run = tokens <= 148 * 8 ? ceil_div(tokens, 148) : round_up(ceil_div(tokens, 148 * 4), 8);
   p.runs = ceil_div(tokens, p.run);
   p.o_token = 256;                       // slot count at 0, joining kernel's counter at 128
   p.o_target = p.o_token + round_up(tokens * 4, 128);
@@ -1338,8 +1381,8 @@ ForwardPlan plan_forward(int64_t tokens, int64_t dim, int64_t vocab) {
   p.block = std::min(tokens, kTokenBlock);
   p.rows_blocks = tokens <= kRowsTokens && (tokens == 1 ? 1 : 4) * dim <= kRowsElems ? std::min<int64_t>(ceil_div(vocab, kRowsThreads / 32 * kRowsPerWarp), 148 * 2) : 0;
   p.parts = p.rows_blocks > 0 ? p.rows_blocks : 2 * ceil_div(vocab, width_for(vocab));
-  p.lanes = 1;
-  while (p.lanes < 8 && p.lanes < tokens) p.lanes <<= 1;
+  p.lanes = 1;                            // rows of a joining block: up to 8 (64 bytes of a partial's row) while there are blocks for all SMs
+  while (p.lanes < 8 && p.lanes * 148 < tokens) p.lanes <<= 1;
   p.join_blocks = (tokens / p.block) * ceil_div(p.block, p.lanes) + ceil_div(tokens % p.block, p.lanes);
   p.o_loss = p.slots.bytes;
   p.o_picked = p.o_loss + round_up(p.join_blocks * 8, 128);

@@ -25,7 +25,10 @@
 // loads into 128-byte-swizzled shared memory.  Operands that run along the other dimension (W for dh, both
 // for dW) are loaded as 64 x 64 boxes and read by the tensor core in their MN-major form, so nothing is
 // transposed in memory.  Two accumulators fill tensor memory (2 x 256 columns): the epilogue of a tile
-// (eight warps, two per lane quadrant) runs under the products of the next.
+// (eight warps, two per lane quadrant) runs under the products of the next.  Measured (B200, nominal 2.25
+// PFLOP/s, cuBLAS 1.38 sustained): 8192 x 4096 x 131072 forward 6.5 ms, 1.36 PFLOP/s, backward 20.1 ms (26.4 TFLOP, 1.31);
+// bound by the power limit.  An epilogue takes 5000 cycles a tile forward and 8000 backward (the exponentials and
+// the chain of a chunk's steps), so widths below about 600 and 1000 are bound by it instead of the products.
 //
 // Outputs of few tiles over a long K (dh of few tokens, dW of few classes) split K over the idle
 // clusters into fp32 slices that a small kernel adds in a fixed order.  No atomics on results: every
@@ -81,23 +84,24 @@ struct XParams {
   const int* token;                              // slot -> token (grad_per_row, and kProduct's rows)
   float* col_part;                               // kGrad: column sums of dl over 32 slots, [slots / 32][col_ld], or null
   int64_t col_ld;
-  // kProduct, kProductT
+  // where the tile goes: kGrad dl, else the result or (splits) fp32 slices
+  void* dst;
+  int64_t ldd;                                   // pitch in elements
   int out_f32;
-  void* out;                                     // kProduct: the result's rows are tokens, not slots, if not null
+  int to_tokens;                                 // kProduct: the result's rows are tokens, not slots
+  float* slices;                                 // kProduct: in place of dst when it splits K itself (pitch: cols)
   const float* acc;                              // added to the result (fp32, pitch ldacc)
   int64_t ldacc;
   int32_t* status;
 };
 
-// kStats stores nothing through shared memory and gets a seventh stage instead; the others stage four bf16
-// (two fp32) chunks per epilogue warp, so that a chunk does not wait for the copy engine to have read the one
-// before the last (with two bf16 chunks a tile's epilogue took 4600 cycles, more than eight K stages' products).
+// kStats stores nothing through shared memory and gets a seventh stage instead.
 template <int kMode, int kBN>
 struct XCfg {
   static constexpr int kBRows = kBN / 2;                         // rows of the second operand per CTA
   static constexpr int kABytes = 128 * kXK * 2, kBBytes = kBRows * kXK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kEpiWarpBytes = kMode == kStats ? 0 : 8192;
+  static constexpr int kEpiWarpBytes = kMode == kStats ? 0 : 4096;   // one 32 x 32 chunk
   static constexpr int kEpiBytes = kXEpiWarps * kEpiWarpBytes;
   static constexpr int kBarBytes = 512;
   static constexpr int kBudget = 227 * 1024 - kEpiBytes - kBarBytes;
@@ -159,22 +163,58 @@ __host__ __device__ __forceinline__ SlotSplit split_slots(int m_tiles, int n_til
   return r;
 }
 
-struct TilePos {
+// A cluster's tiles.  They go down a group of group_m tile rows before the next column: the first operand's rows
+// of the group stay in L2 while the second operand streams past once per group.  The next tile is found by
+// adding (the divisions of finding it afresh took 400 cycles of every epilogue warp and tile); a
+// product that is split has about one unit per cluster, and divides.
+struct TileWalk {
   int m, n, split;
+  int unit, step;
+  int grp, in_grp, rows;           // group, tile row in it, tile rows of it
+  int dn, dm;                      // a step in columns and rows of a whole group
+
+  __device__ __forceinline__ void start(const XParams& g, int first, int stride) {
+    unit = first;
+    step = stride;
+    const int tile = unit / g.splits;
+    split = unit - tile * g.splits;
+    const int span = g.group_m * g.n_tiles;
+    grp = tile / span;
+    locate(g, tile - grp * span);
+  }
+  __device__ __forceinline__ void locate(const XParams& g, int rem) {
+    rows = max(1, min(g.group_m, g.m_tiles - grp * g.group_m));
+    n = rem / rows;
+    in_grp = rem - n * rows;
+    m = grp * g.group_m + in_grp;
+    dn = step / rows;
+    dm = step - dn * rows;
+  }
+  __device__ __forceinline__ void advance(const XParams& g) {
+    if (g.splits > 1) {
+      start(g, unit + step, step);
+      return;
+    }
+    unit += step;
+    in_grp += dm;
+    n += dn;
+    if (in_grp >= rows) {
+      in_grp -= rows;
+      ++n;
+    }
+    if (n >= g.n_tiles) {          // into a later group
+      int rem = n * rows + in_grp;
+      do {
+        rem -= rows * g.n_tiles;
+        ++grp;
+        rows = max(1, min(g.group_m, g.m_tiles - grp * g.group_m));
+      } while (rem >= rows * g.n_tiles && grp * g.group_m < g.m_tiles);
+      locate(g, rem);
+    } else {
+      m = grp * g.group_m + in_grp;
+    }
+  }
 };
-// Tiles go down a group of group_m tile rows before the next column: the first operand's rows of the
-// group stay in L2 while the second operand streams past once per group.
-__device__ __forceinline__ TilePos tile_at(const XParams& g, int unit) {
-  TilePos t;
-  const int tile = unit / g.splits;
-  t.split = unit - tile * g.splits;
-  const int span = g.group_m * g.n_tiles;
-  const int grp = tile / span, rem = tile - grp * span;
-  const int rows = min(g.group_m, g.m_tiles - grp * g.group_m);
-  t.n = rem / rows;
-  t.m = grp * g.group_m + rem - t.n * rows;
-  return t;
-}
 
 // bias of the 32 columns from c on (columns behind the last read as zero)
 __device__ __forceinline__ void add_bias(const XParams& g, int c, float (&v)[32]) {
@@ -225,46 +265,50 @@ __device__ __forceinline__ float column_sums(const float (&v)[32], int lane) {
   return w[0];
 }
 
-// One 32 x 32 chunk (a row per lane) to a swizzled staging tile and from there with one tiled TMA
-// store, clipped at the matrix edges.  `buf`: the warp's 8 KB, four 2-KB tiles of bf16 or two of fp32 in turn.
-__device__ __forceinline__ void store_chunk_bf16(const CUtensorMap* map, uint8_t* buf, uint32_t& n_emit, int lane, int row, int col,
-                                                 const float (&v)[32]) {
-  uint8_t* tile = buf + (n_emit & 3u) * 2048;
-  if (lane == 0) bulk_wait_read<3>();
-  __syncwarp();
+// One 32 x 32 chunk (a row per lane) through the warp's staging tile to whole 64- or 128-byte pieces of
+// rows.  Plain stores: handing the tile to the copy engine (proxy fence, TMA store, wait for the tile) was no
+// faster on many tokens and 6 % slower on few (16 tokens, 131072 x 4096: backward 926 against 870 us).  Columns end at a multiple of 8 (of dl at its pitch).  `token`: rows of the result by slot, or null.
+struct Dest {
+  uint8_t* p;
+  int64_t pitch;                   // bytes
+  int row_end, col_end;
+  const int* token;
+};
+template <bool kF32>
+__device__ __forceinline__ void store_chunk(const Dest& d, uint8_t* tile, int lane, int row0, int col, const float (&v)[32]) {
+  constexpr int kPiece = kF32 ? 8 : 4;            // 16-byte pieces of a row of the chunk
+  __syncwarp();                                   // the chunk before has been read
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t w[4];
+  for (int j = 0; j < kPiece; ++j) {
+    uint4 q;
+    if (kF32) {
+      q = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+    } else {
+      uint32_t w[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * t], v[8 * j + 2 * t + 1]);
-      w[t] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int t = 0; t < 4; ++t) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * t], v[8 * j + 2 * t + 1]);
+        w[t] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      q = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(tile + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    const int at = kF32 ? j ^ (lane & 7) : j ^ ((lane >> 1) & 3);        // conflict-free both ways
+    *reinterpret_cast<uint4*>(tile + lane * (kPiece * 16) + (at << 4)) = q;
   }
-  fence_async_smem();
   __syncwarp();
-  if (lane == 0) {
-    tma_store_2d(map, smem_u32(tile), col, row);
-    bulk_commit();
-  }
-  ++n_emit;
-}
-__device__ __forceinline__ void store_chunk_f32(const CUtensorMap* map, uint8_t* buf, uint32_t& n_emit, int lane, int row, int col,
-                                                const float (&v)[32]) {
-  uint8_t* tile = buf + (n_emit & 1u) * 4096;
-  if (lane == 0) bulk_wait_read<1>();
-  __syncwarp();
+  const int piece = lane & (kPiece - 1);
+  const int c = col + piece * (kF32 ? 4 : 8);
+  uint8_t* base = d.p + (int64_t)c * (kF32 ? 4 : 2);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<float4*>(tile + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  fence_async_smem();
-  __syncwarp();
-  if (lane == 0) {
-    tma_store_2d(map, smem_u32(tile), col, row);
-    bulk_commit();
+  for (int i = 0; i < kPiece; ++i) {
+    const int r = i * (32 / kPiece) + lane / kPiece, row = row0 + r;
+    const int at = kF32 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3);
+    const uint4 q = *reinterpret_cast<const uint4*>(tile + r * (kPiece * 16) + (at << 4));
+    if (row < d.row_end && c < d.col_end) {
+      const int to = d.token != nullptr ? __ldcg(d.token + row) : row;
+      *reinterpret_cast<uint4*>(base + (int64_t)to * d.pitch) = q;
+    }
   }
-  ++n_emit;
 }
 
 // The wait for a tcgen05.ld that was issued before other work: its registers pass through, so that nothing
@@ -286,33 +330,10 @@ __device__ __forceinline__ void scale_to_log2(float (&v)[32], float ref) {
   for (int j = 0; j < 32; j += 2) fma(Pack<2>::of(v + j), l, m).to(v + j);
 }
 
-// The same chunk to rows that are not neighbours: each lane its own (columns are a multiple of 8).
-__device__ __forceinline__ void store_row_chunk(void* row, int out_f32, int col, int cols, const float (&v)[32]) {
-  if (row == nullptr) return;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (col + 8 * j < cols) {
-      if (out_f32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(row) + col + 8 * j);
-        p[0] = make_float4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
-        p[1] = make_float4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
-      } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * t], v[8 * j + 2 * t + 1]);
-          w[t] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(row) + col + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
-  }
-}
-
 template <int kMode, int kBN>
 __global__ void __launch_bounds__(kXThreads, 1)
 xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                 const __grid_constant__ CUtensorMap map_packed, const __grid_constant__ CUtensorMap map_d, const XParams gp) {
+                 const __grid_constant__ CUtensorMap map_packed, const XParams gp) {
   using C = XCfg<kMode, kBN>;
   XParams g = gp;
   constexpr bool kAMn = kMode == kProductT, kBMn = kMode == kProduct || kMode == kProductT;
@@ -340,8 +361,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   if (threadIdx.x == 32) {
     tma_prefetch_map(&map_a);
     tma_prefetch_map(&map_b);
-    if (kMode != kProduct || gp.split_clusters > 0) tma_prefetch_map(&map_packed);
-    if (kMode != kStats) tma_prefetch_map(&map_d);
+    if (kMode != kProduct) tma_prefetch_map(&map_packed);
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -384,7 +404,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       g.slice_rows = g.m_tiles * kXM;
     }
   }
-  const bool sliced = kMode == kProduct && (g.splits > 1 || g.few);   // fp32 slices (map_packed), summed by another kernel
+  const bool sliced = kMode == kProduct && (g.splits > 1 || g.few);   // fp32 slices, summed by another kernel
   const CUtensorMap* tma_a = (kMode == kStats || kMode == kGrad) && !dense ? &map_packed : &map_a;
   const CUtensorMap* tma_b = kMode == kProductT && !dense ? &map_packed : &map_b;
   const int units = g.m_tiles * g.n_tiles * g.splits;
@@ -397,8 +417,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int unit = cluster_id; ok && unit < units; unit += num_clusters) {
-        const TilePos t = tile_at(g, unit);
+      TileWalk t;
+      for (t.start(g, cluster_id, num_clusters); ok && t.unit < units; t.advance(g)) {
         const int ks0 = t.split * g.ks_per_split, ks1 = min(ks0 + g.ks_per_split, g.k_stages);
         const int row_a = t.m * kXM + (int)rank * 128, row_b = t.n * kBN + (int)rank * C::kBRows;
         for (int ks = ks0; ks < ks1; ++ks) {
@@ -437,7 +457,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       bool ok = true;
       int it = 0;
       for (int unit = cluster_id; ok && unit < units; unit += num_clusters, ++it) {
-        const int split = unit % g.splits;
+        const int split = g.splits > 1 ? unit % g.splits : 0;
         const int ks0 = split * g.ks_per_split, ks1 = min(ks0 + g.ks_per_split, g.k_stages);
         const int a = it & 1;
         ok = mbar_wait(bar_tmem_empty + 8 * a, ((it >> 1) & 1) ^ 1u, abort_flag, g.status, 22);
@@ -470,24 +490,43 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     // ------------------------------ epilogue (each CTA) ------------------------------
     const int quad = warp & 3, half = (warp - 4) >> 2;
     uint8_t* buf = smem + C::kEpi0 + (warp - 4) * C::kEpiWarpBytes;
-    uint32_t n_emit = 0;
     // a scalar gradient of the loss scales the products (and db), one per token is part of dl
     float scale = 1.f;
-    if (kMode != kStats && !g.grad_per_row) scale = g.mean ? (slots > 0 ? __ldg(g.grad) / (float)slots : 0.f) : __ldg(g.grad);
+    if (kMode != kStats && !g.grad_per_row) scale = g.mean ? (slots > 0 ? __ldcg(g.grad) / (float)slots : 0.f) : __ldcg(g.grad);
     int it = 0;
-    for (int unit = cluster_id; unit < units; unit += num_clusters, ++it) {
-      const TilePos t = tile_at(g, unit);
+    TileWalk t;
+    t.start(g, cluster_id, num_clusters);
+    // What a row brings to its tile (target, lse, gradient) is loaded a tile ahead.  Through L2: the kernel may
+    // have been resident before its predecessor wrote them, which the read-only path must not see.
+    int row0 = 0, slot = 0, y = -1;
+    bool row_ok = false;
+    float lse = 0.f, gr = 1.f;
+    const auto look = [&]() {
+      row0 = t.m * kXM + (int)rank * 128 + quad * 32;
+      const int row = row0 + lane;
+      slot = kMode == kGrad && g.few ? row & (kFew - 1) : row;
+      row_ok = t.unit < units && row < g.rows && (kMode != kGrad || slot < slots);
+      if (kMode == kStats || kMode == kGrad) {
+        y = row_ok ? __ldcg(g.target + slot) : -1;
+        if (kMode == kGrad) {
+          lse = row_ok ? __ldcg(g.lse + slot) : 0.f;
+          if (g.grad_per_row) gr = row_ok ? __ldcg(g.grad + __ldcg(g.token + slot)) : 0.f;
+        }
+      }
+    };
+    look();
+    for (; t.unit < units; ++it) {
       const int a = it & 1;
-      int ok = 1;
-      if (lane == 0) ok = mbar_wait(bar_tmem_full + 8 * a, (uint32_t)((it >> 1) & 1), abort_flag, g.status, 24) ? 1 : 0;
-      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-      if (!ok) break;
+      const int my_row0 = row0, row = row0 + lane, n_tile = t.n, split = t.split, my_y = y;
+      const bool my_ok = row_ok;
+      const float my_lse = lse, my_gr = gr;
+      t.advance(g);
+      look();
+      const bool ok = mbar_wait(bar_tmem_full + 8 * a, (uint32_t)((it >> 1) & 1), abort_flag, g.status, 24);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
       tc_fence_after();
       const uint32_t acc = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(a * kBN + half * C::kHalf);
-      const int row0 = t.m * kXM + (int)rank * 128 + quad * 32, row = row0 + lane;
-      const int slot = kMode == kGrad && g.few ? row & (kFew - 1) : row;
-      const bool row_ok = row < g.rows && (kMode != kGrad || slot < slots);
-      const int colbase = t.n * kBN + half * C::kHalf;
+      const int colbase = n_tile * kBN + half * C::kHalf;
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
@@ -495,17 +534,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       };
       if (kMode == kStats || kMode == kGrad) {
         // the target's column in this warp's part of the tile; anything outside [0, cols) never matches
-        const int yc = row_ok ? __ldg(g.target + slot) - g.col0 : -1;
+        const int yc = my_ok ? my_y - g.col0 : -1;
         const int mine = yc >= colbase && yc < colbase + C::kHalf && yc < g.cols ? yc - colbase : -1;
         // dl's rows up to the end of the last K stage that reads them are written (as zeros)
         const int row_end = kMode == kGrad ? (g.rows + kXK - 1) / kXK * kXK : g.rows;
         float m = -INFINITY, s = 0.f, x_y = 0.f;
-        float lse = 0.f, gr = 0.f;
-        if (kMode == kGrad) {
-          lse = row_ok ? __ldg(g.lse + slot) : 0.f;
-          gr = g.grad_per_row ? (row_ok ? __ldg(g.grad + __ldg(g.token + slot)) : 0.f) : 1.f;
-        }
-        const bool all_ok = __all_sync(0xFFFFFFFFu, row_ok);
+        const bool all_ok = __all_sync(0xFFFFFFFFu, my_ok);
+        const Dest dest{static_cast<uint8_t*>(g.dst), g.ldd * 2, min(row_end, gp.rows), (g.cols + 7) / 8 * 8, nullptr};
         constexpr int kN = C::kHalf / 32;
         uint32_t r[2][32];
         tc_ld32(acc, r[0]);
@@ -515,7 +550,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           if (c + 1 < kN) tc_ld32(acc + (uint32_t)((c + 1) * 32), r[(c + 1) & 1]);    // under this chunk's work
           else release();
           const int col = colbase + c * 32;
-          if (col >= g.cols || row0 >= row_end) continue;     // warp-uniform
+          if (col >= g.cols || my_row0 >= row_end) continue;     // warp-uniform
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[c & 1][j]);
@@ -557,13 +592,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             m = mn;
           } else {
-            if (fabsf(lse) < kFar) {
-              scale_to_log2(v, lse * kLog2e);
+            if (fabsf(my_lse) < kFar) {
+              scale_to_log2(v, my_lse * kLog2e);
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = exp2_fast(v[j]);
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = exp2_fast((v[j] - lse) * kLog2e);
+              for (int j = 0; j < 32; ++j) v[j] = exp2_fast((v[j] - my_lse) * kLog2e);
             }
             if (__any_sync(0xFFFFFFFFu, (mine >> 5) == c)) {
 #pragma unroll
@@ -572,32 +607,34 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             if (g.grad_per_row) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= gr;
+              for (int j = 0; j < 32; ++j) v[j] *= my_gr;
             }
             if (!all_ok) {                                    // rows without a token: zeros, whatever the tile holds there
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = row_ok ? v[j] : 0.f;
+              for (int j = 0; j < 32; ++j) v[j] = my_ok ? v[j] : 0.f;
             }
-            if (g.col_part != nullptr && (!g.few || row0 < kFew)) {
+            if (g.col_part != nullptr && (!g.few || my_row0 < kFew)) {
               const float sum = column_sums(v, lane) * scale;
-              if (col + lane < g.cols) g.col_part[(int64_t)(row0 >> 5) * g.col_ld + col + lane] = sum;
+              if (col + lane < g.cols) g.col_part[(int64_t)(my_row0 >> 5) * g.col_ld + col + lane] = sum;
             }
-            if (g.few && row0 >= kFew) {                      // what the rows' first bf16 lose
+            if (g.few && my_row0 >= kFew) {                      // what the rows' first bf16 lose
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
             }
-            store_chunk_bf16(&map_d, buf, n_emit, lane, row0, col, v);
+            store_chunk<false>(dest, buf, lane, my_row0, col, v);
           }
         }
-        if (kMode == kStats && row_ok) {
-          g.part[(int64_t)(2 * t.n + half) * gp.rows + row] = make_float2(m, s);
+        if (kMode == kStats && my_ok) {
+          g.part[(int64_t)(2 * n_tile + half) * gp.rows + row] = make_float2(m, s);
           if (mine >= 0) g.picked[row] = x_y;
         }
       } else {
-        const bool nothing = t.split * g.ks_per_split >= g.k_stages;    // no stage of K: no product was issued
-        void* out_row = nullptr;
-        if (kMode == kProduct && g.out != nullptr && !dense && row_ok)
-          out_row = static_cast<uint8_t*>(g.out) + (int64_t)__ldg(g.token + row) * g.cols * (g.out_f32 ? 4 : 2);
+        const bool nothing = split * g.ks_per_split >= g.k_stages;      // no stage of K: no product was issued
+        const bool f32 = sliced || g.out_f32;
+        const int64_t first = sliced ? (int64_t)split * g.slice_rows * g.cols : kMode == kProductT ? (int64_t)split * g.slice_rows * g.ldd : 0;
+        const int64_t pitch = sliced ? g.cols : g.ldd;
+        const Dest dest{static_cast<uint8_t*>(sliced ? static_cast<void*>(g.slices) : g.dst) + first * (f32 ? 4 : 2), pitch * (f32 ? 4 : 2), g.rows,
+                        g.cols, !sliced && g.to_tokens && !dense ? g.token : nullptr};
         constexpr int kN = C::kHalf / 32;
         uint32_t r[2][32];
         tc_ld32(acc, r[0]);
@@ -607,11 +644,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           if (c + 1 < kN) tc_ld32(acc + (uint32_t)((c + 1) * 32), r[(c + 1) & 1]);
           else release();
           const int col = colbase + c * 32;
-          if (col >= g.cols || row0 >= g.rows) continue;
+          if (col >= g.cols || my_row0 >= g.rows) continue;
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = nothing ? 0.f : __uint_as_float(r[c & 1][j]) * scale;
-          if (g.acc != nullptr && row_ok && !sliced) {         // columns are a multiple of 8: whole vectors
+          if (g.acc != nullptr && my_ok && !sliced) {         // columns are a multiple of 8: whole vectors
             const float4* p = reinterpret_cast<const float4*>(g.acc + (int64_t)row * g.ldacc + col);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -621,16 +658,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
               }
             }
           }
-          const int srow = row0 + t.split * g.slice_rows;
-          if (sliced) store_chunk_f32(&map_packed, buf, n_emit, lane, srow, col, v);
-          else if (kMode == kProduct && g.out != nullptr && !dense) store_row_chunk(out_row, g.out_f32, col, g.cols, v);
-          else if (g.out_f32) store_chunk_f32(&map_d, buf, n_emit, lane, srow, col, v);
-          else store_chunk_bf16(&map_d, buf, n_emit, lane, srow, col, v);
+          if (f32) store_chunk<true>(dest, buf, lane, my_row0, col, v);
+          else store_chunk<false>(dest, buf, lane, my_row0, col, v);
         }
       }
     }
-    if (lane == 0) bulk_wait_all<0>();
-    __syncwarp();
   }
 
   // ------------------------------ teardown ------------------------------
@@ -706,7 +738,7 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
   } else {
 #pragma unroll 8
     for (int t = threadIdx.x; t < p.tokens; t += kPackThreads) {
-      const int c = __ldg(reinterpret_cast<const long long*>(p.target) + t) != p.ignore;
+      const int c = __ldcg(reinterpret_cast<const long long*>(p.target) + t) != p.ignore;
       all += c;
       if (t < t0) before += c;
     }
@@ -721,7 +753,7 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
   }
   for (int base = t0; base < t1; base += kPackThreads) {
     const int t = base + (int)threadIdx.x;
-    const int64_t y = t < t1 ? __ldg(reinterpret_cast<const long long*>(p.target) + t) : p.ignore;
+    const int64_t y = t < t1 ? __ldcg(reinterpret_cast<const long long*>(p.target) + t) : p.ignore;
     const bool counted = t < t1 && y != p.ignore;
     const uint32_t votes = __ballot_sync(0xFFFFFFFFu, counted);
     __syncthreads();                              // red and source of the round before are read
@@ -749,7 +781,7 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
         for (int k = 0; k < 4; ++k) {
           const int64_t c = c0 + k * kPackThreads;
           const int i = (int)(c / vecs);
-          if (i < total) v[k] = __ldg(reinterpret_cast<const uint4*>(p.h + (int64_t)source[i] * p.ldh) + (c - (int64_t)i * vecs));
+          if (i < total) v[k] = __ldcg(reinterpret_cast<const uint4*>(p.h + (int64_t)source[i] * p.ldh) + (c - (int64_t)i * vecs));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -786,7 +818,8 @@ __global__ void __launch_bounds__(kPackThreads) xent_pack_kernel(const PackParam
 }
 
 // The forward statistics of one to four tokens: reading W is all there is to it, and whole rows in a row
-// read better than the tensor core's 128-byte columns of 256 rows (131072 x 4096, one token: FIGURES).  A warp
+// read better than the tensor core's 128-byte columns of 256 rows (131072 x 4096, one token: 184 against 245 us; the
+// bytes' floor is 163).  A warp
 // takes four neighbouring rows of W at a time, the tokens' states wait in shared memory as bf16; products
 // and sums in fp32.  One partial (maximum, sum) per block and token.
 constexpr int kRowsThreads = 256, kRowsPerWarp = 4, kRowsTokens = 4;
@@ -1153,10 +1186,9 @@ int bf16_map(CUtensorMap* map, const Operand& o, int box_inner, int box_outer, C
                               (uint32_t)box_inner, (uint32_t)box_outer, sw);
 }
 
-// `packed`: the counted tokens' rows of h, read in place of operand a (kStats, kGrad) or b (kProductT); for
-// kProduct the fp32 slices.
+// `packed`: the counted tokens' rows of h, read in place of operand a (kStats, kGrad) or b (kProductT).
 template <int kMode, int kBN>
-int launch_width(const Operand& a, const Operand& b, const Operand& packed, void* out, int64_t ldo, XParams g, int64_t k, cudaStream_t stream) {
+int launch_width(const Operand& a, const Operand& b, const Operand& packed, XParams g, int64_t k, cudaStream_t stream) {
   using C = XCfg<kMode, kBN>;
   constexpr bool kAMn = kMode == kProductT, kBMn = kMode == kProduct || kMode == kProductT;
   const int resident = xent_clusters<kMode, kBN>();
@@ -1175,20 +1207,12 @@ int launch_width(const Operand& a, const Operand& b, const Operand& packed, void
   }
   // the first operand's rows of a group: 32 MB, a quarter of L2
   g.group_m = (int)std::min<int64_t>(g.m_tiles, std::max<int64_t>(1, (32ll << 20) / ((int64_t)kXM * 2 * std::max<int64_t>(k, 1))));
-  CUtensorMap map_a, map_b, map_packed = {}, map_d = {};
+  CUtensorMap map_a, map_b, map_packed = {};
   int rc = kAMn ? bf16_map(&map_a, a, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_a, a, kXK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == FP4T_OK)
     rc = kBMn ? bf16_map(&map_b, b, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_b, b, kXK, C::kBRows, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == FP4T_OK && kMode == kProduct && g.split_clusters > 0)
-    rc = encode_tensor_map_2d(&map_packed, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, packed.p, (uint64_t)packed.inner, (uint64_t)packed.outer,
-                              (uint64_t)packed.ld * 4, 32u, 32u, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == FP4T_OK && kMode != kProduct)
     rc = kBMn ? bf16_map(&map_packed, packed, 64, kXK, CU_TENSOR_MAP_SWIZZLE_128B) : bf16_map(&map_packed, packed, kXK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == FP4T_OK && kMode != kStats) {
-    const uint64_t rows = g.splits > 1 ? (uint64_t)g.splits * g.slice_rows : (uint64_t)g.rows;
-    rc = encode_tensor_map_2d(&map_d, g.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, (uint64_t)g.cols, rows,
-                              (uint64_t)ldo * (g.out_f32 ? 4 : 2), 32u, 32u, g.out_f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-  }
   if (rc != FP4T_OK) return rc;
   const int64_t units = kMode == kProduct && g.split_clusters > 0 ? clusters : (int64_t)g.m_tiles * g.n_tiles * g.splits;
   cudaLaunchConfig_t cfg = {};
@@ -1203,13 +1227,12 @@ int launch_width(const Operand& a, const Operand& b, const Operand& packed, void
   pdl_attribute(&attr[1]);
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  FP4T_CUDA(cudaLaunchKernelEx(&cfg, xent_gemm_kernel<kMode, kBN>, map_a, map_b, map_packed, map_d, g));
+  FP4T_CUDA(cudaLaunchKernelEx(&cfg, xent_gemm_kernel<kMode, kBN>, map_a, map_b, map_packed, g));
   return FP4T_OK;
 }
 template <int kMode>
-int launch_xent(int bn, const Operand& a, const Operand& b, const Operand& packed, void* out, int64_t ldo, const XParams& g, int64_t k,
-                cudaStream_t stream) {
-  return bn == 128 ? launch_width<kMode, 128>(a, b, packed, out, ldo, g, k, stream) : launch_width<kMode, 256>(a, b, packed, out, ldo, g, k, stream);
+int launch_xent(int bn, const Operand& a, const Operand& b, const Operand& packed, const XParams& g, int64_t k, cudaStream_t stream) {
+  return bn == 128 ? launch_width<kMode, 128>(a, b, packed, g, k, stream) : launch_width<kMode, 256>(a, b, packed, g, k, stream);
 }
 
 template <typename... Args, typename... Actual>
@@ -1266,11 +1289,14 @@ int run_dh(const Operand& dl, const Operand& w, int64_t tokens, int64_t dim, int
   g.out_f32 = out_f32;
   g.acc = acc;
   g.ldacc = dim;
-  g.out = to_tokens ? out : nullptr;
+  g.dst = out;
+  g.ldd = dim;
+  g.to_tokens = to_tokens;
+  g.slices = slices;
   const int bn = width_for(dim);
   split_clusters = std::min(split_clusters, bn == 128 ? xent_clusters<kProduct, 128>() : xent_clusters<kProduct, 256>());
   g.split_clusters = slice_rows > 0 ? split_clusters : 0;      // (the kernel's launch refuses when none can be resident)
-  int rc = launch_xent<kProduct>(bn, dl, w, Operand{slices, slice_rows, dim, dim}, out, dim, g, vc, stream);
+  int rc = launch_xent<kProduct>(bn, dl, w, Operand{}, g, vc, stream);
   if (rc != FP4T_OK || g.split_clusters <= 0) return rc;
   SliceParams p = {};
   p.slices = slices;
@@ -1304,7 +1330,9 @@ int run_dw(const Cut& cut, const Operand& dl, const Operand& h, const Operand& p
   g.ks_per_split = cut.ks_per_split;
   g.out_f32 = cut.splits > 1 ? 1 : out_f32;
   g.slice_rows = (int)cut.slice_rows;
-  int rc = launch_xent<kProductT>(cut.bn, dl, h, packed, cut.splits > 1 ? slices : out, dim, g, dl.outer, stream);
+  g.dst = cut.splits > 1 ? slices : out;
+  g.ldd = dim;
+  int rc = launch_xent<kProductT>(cut.bn, dl, h, packed, g, dl.outer, stream);
   if (rc != FP4T_OK || cut.splits == 1) return rc;
   SliceParams p = {};
   p.slices = slices;
@@ -1509,7 +1537,7 @@ extern "C" int fp4t_linear_xent_forward(const void* h, int64_t ldh, const void* 
       rc = launch_small_shared(kern, (int)p.rows_blocks, kRowsThreads, (tokens == 1 ? 1 : 4) * dim * 2, s, r);
     } else
       rc = launch_xent<kStats>(width_for(vocab), Operand{static_cast<const __nv_bfloat16*>(h) + t0 * ldh, rows, dim, ldh}, Operand{w, vocab, dim, ldw},
-                             Operand{sl.packed + t0 * dim, rows, dim, dim}, nullptr, 0, g, dim, s);
+                             Operand{sl.packed + t0 * dim, rows, dim, dim}, g, dim, s);
     if (rc != FP4T_OK) return rc;
     JoinParams j = {};
     j.part = g.part;
@@ -1599,7 +1627,9 @@ extern "C" int fp4t_linear_xent_backward(const float* grad_loss, const void* h, 
     g.col_part = db ? reinterpret_cast<float*>(ws + p.o_cols) : nullptr;
     g.col_ld = p.ld;
     g.status = status;
-    rc = launch_xent<kGrad>(width_for(vc), hop, wop, packed, dl, p.ld, g, dim, s);
+    g.dst = dl;
+    g.ldd = p.ld;
+    rc = launch_xent<kGrad>(width_for(vc), hop, wop, packed, g, dim, s);
     if (rc != FP4T_OK) return rc;
     if (dh) {
       const bool last = i == p.pieces - 1;

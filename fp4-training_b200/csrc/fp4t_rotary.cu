@@ -15,10 +15,13 @@
 //
 // A head is held by a group of 1 to 32 lanes, up to eight pairs (two 16-byte vectors of bf16) a lane, so the
 // norm is a shuffle reduction inside the group and every element is read and written once:
-// HBM-bound (forward 4 bytes per bf16 element, norm backward 6).  A group walks heads of ONE token,
-// queries and keys, with the cosines and sines of its pairs in registers: no shared memory, no barrier, and
-// the trigonometry is paid once per token, not per head.  Several heads' vectors are loaded before the
-// first is worked on, the first ones before the angles are computed.
+// HBM-bound (forward 4 bytes per bf16 element, norm backward 6).  Measured (B200, copy bandwidth 6.57 TB/s):
+// 65536 tokens x 40 heads x 128 bf16 rotation 204 us, 6.58 TB/s; 32768 tokens with norms forward 113 us, 5.9 TB/s,
+// backward 183 us, 5.5 TB/s (bound by the chain of two reductions per head at 16 warps per SM).
+//
+// A group walks heads of ONE token, queries and keys, with the cosines and sines of its pairs in registers: no
+// table, no barrier, and the trigonometry is paid once per token, not per head.  Several heads' vectors are under way
+// before the first is worked on, the first ones before the angles are computed.
 #include <algorithm>
 
 #include "fp4t_common.cuh"
@@ -192,6 +195,13 @@ struct LaneView {
       r.b[s].load(x + eb[s]);
     }
   }
+  // the same from two 16-byte vectors (V = 8, bf16)
+  static __device__ __forceinline__ void from_shared(const uint4& a, const uint4& b, Head& r) {
+    uint32_t* w = r.a[0].u;
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w = r.b[0].u;
+    w[0] = b.x; w[1] = b.y; w[2] = b.z; w[3] = b.w;
+  }
   // A lane's pairs as packs: first members in a, second ones in b; pack j belongs to chunk slot(j).
   static constexpr int W = V == 1 ? 1 : 2, kPacks = 8 / W;
   static __device__ __forceinline__ constexpr int slot(int j) { return j * W / V; }
@@ -298,16 +308,29 @@ struct LaneView {
     }
   }
 };
+// Asynchronous 16-byte copies to shared memory, waited for by the thread that started them.
+__device__ __forceinline__ void copy_ahead(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_ahead_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copy_ahead_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
 // Forward (and the plain rotation's backward).  A warp works on 32 / group tokens and one chunk of
-// their heads; kBatch heads are in flight per lane, each one's registers are loaded again as soon as it is
-// unpacked.  Blocks in the order of the tokens, not persistent: what runs at one time then touches one
+// their heads; kBatch heads are in flight per lane, or (norm, bf16 in whole 16-byte vectors) kDepth heads through
+// shared memory, each lane's own copies, which leaves registers for the factors: 121 -> 113 us, without the norm it
+// made no difference.  Blocks in the order of the tokens, not persistent: what runs at one time then touches one
 // stretch of memory (an even share of far-apart stretches for each resident warp took 271 instead of 204 us on
 // 65536 tokens).  With the norm the weights are multiplied into the
 // cosines and sines once per token and tensor, y = r (x_a (w_a c) - x_b (w_b s), x_a (w_a s) + x_b (w_b c)), six packed
 // instructions for two pairs.
 template <typename T, int V, bool kHalf, bool kNorm>
 __global__ void __launch_bounds__(kRotThreads, 4) qk_rotary_kernel(const RotParams p) {
-  constexpr int kBatch = sizeof(T) == 4 ? 2 : V == 1 ? 2 : 4;      // 32 registers of raw vectors
+  constexpr bool kAhead = kNorm && sizeof(T) == 2 && V == 8;
+  constexpr int kBatch = sizeof(T) == 4 ? 2 : V == 1 ? 2 : 4, kDepth = 4;      // 32 registers of raw vectors
+  __shared__ uint4 ring[kAhead ? kDepth : 1][2][kAhead ? kRotThreads : 1];
   using View = LaneView<T, V, kHalf>;
   using P = typename View::P;
   constexpr int N = View::kPacks;
@@ -334,8 +357,19 @@ __global__ void __launch_bounds__(kRotThreads, 4) qk_rotary_kernel(const RotPara
     const T* x = static_cast<const T*>(p.x[which].p) + b * p.x[which].sb + l * p.x[which].st + first * xs;
     T* y = static_cast<T*>(p.y[which].p) + b * p.y[which].sb + l * p.y[which].st + first * ys;
     typename View::Head raw[kBatch];
+    if constexpr (kAhead) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) view.load(x + min(u, last - 1 - first) * xs, raw[u]);
+      for (int u = 0; u < kDepth; ++u) {
+        if (first + u < last) {
+          copy_ahead(&ring[u][0][threadIdx.x], x + u * xs + view.ea[0]);
+          copy_ahead(&ring[u][1][threadIdx.x], x + u * xs + view.eb[0]);
+        }
+        copy_ahead_commit();
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) view.load(x + min(u, last - 1 - first) * xs, raw[u]);
+    }
     if (!have_angles) {
       view.angles(p, lane, b, l, p.sign, cf, sf);
       have_angles = true;
@@ -358,35 +392,51 @@ __global__ void __launch_bounds__(kRotThreads, 4) qk_rotary_kernel(const RotPara
         kb[j] = mul(sn, minus);
       }
     }
-    for (int h = first; h < last; h += kBatch) {
+    const auto work = [&](const typename View::Head& head, T* out) {
+      P a[N], d[N];
+      view.expand(head, a, d);
+      P r = P::all(1.f);
+      if constexpr (kNorm) r = P::all(rsqrtf(group_sum(view.sum_of_products(a, a, d, d), p.group) * p.inv_dim + p.eps));
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (h + u < last) {                               // warp-uniform
-          P a[N], d[N];
-          view.expand(raw[u], a, d);
-          P r = P::all(1.f);
-          if constexpr (kNorm) r = P::all(rsqrtf(group_sum(view.sum_of_products(a, a, d, d), p.group) * p.inv_dim + p.eps));
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            P ya = a[j], yb = d[j];
-            if (view.turns[View::slot(j)]) {
-              ya = fma(d[j], kb[j], mul(a[j], ka[j]));
-              yb = fma(d[j], lb[j], mul(a[j], la[j]));
-            } else if constexpr (kNorm) {                 // c = 1: the factors are the weights
-              ya = mul(a[j], ka[j]);
-              yb = mul(d[j], lb[j]);
-            }
-            a[j] = kNorm ? mul(ya, r) : ya;
-            d[j] = kNorm ? mul(yb, r) : yb;
-          }
-          if (token_live) view.store(y + u * ys, a, d);
+      for (int j = 0; j < N; ++j) {
+        P ya = a[j], yb = d[j];
+        if (view.turns[View::slot(j)]) {
+          ya = fma(d[j], kb[j], mul(a[j], ka[j]));
+          yb = fma(d[j], lb[j], mul(a[j], la[j]));
+        } else if constexpr (kNorm) {                     // c = 1: the factors are the weights
+          ya = mul(a[j], ka[j]);
+          yb = mul(d[j], lb[j]);
         }
+        a[j] = kNorm ? mul(ya, r) : ya;
+        d[j] = kNorm ? mul(yb, r) : yb;
       }
-      x += kBatch * xs;
-      y += kBatch * ys;
-      if (h + kBatch < last) {
+      if (token_live) view.store(out, a, d);
+    };
+    if constexpr (kAhead) {
+      for (int h = first; h < last; ++h) {
+        const int slot = (h - first) & (kDepth - 1);
+        copy_ahead_wait<kDepth - 1>();
+        view.from_shared(ring[slot][0][threadIdx.x], ring[slot][1][threadIdx.x], raw[0]);
+        work(raw[0], y);
+        if (h + kDepth < last) {
+          copy_ahead(&ring[slot][0][threadIdx.x], x + kDepth * xs + view.ea[0]);
+          copy_ahead(&ring[slot][1][threadIdx.x], x + kDepth * xs + view.eb[0]);
+        }
+        copy_ahead_commit();
+        x += xs;
+        y += ys;
+      }
+    } else {
+      for (int h = first; h < last; h += kBatch) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) view.load(x + min(u, last - 1 - h - kBatch) * xs, raw[u]);
+        for (int u = 0; u < kBatch; ++u)
+          if (h + u < last) work(raw[u], y + u * ys);     // warp-uniform
+        x += kBatch * xs;
+        y += kBatch * ys;
+        if (h + kBatch < last) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) view.load(x + min(u, last - 1 - h - kBatch) * xs, raw[u]);
+        }
       }
     }
   }
@@ -396,7 +446,12 @@ __global__ void __launch_bounds__(kRotThreads, 4) qk_rotary_kernel(const RotPara
 // persistent: they are kept over all its tokens and reduced once.
 template <typename T, int V, bool kHalf>
 __global__ void __launch_bounds__(kRotThreads, 4) qk_norm_rotary_bwd_kernel(const RotParams p) {
-  constexpr int kBatch = sizeof(T) == 4 || V == 1 ? 1 : 2;         // 32 registers of raw vectors
+  // bf16 in whole 16-byte vectors is copied to shared memory kDepth heads ahead, each lane its own (nothing to wait for
+  // but its own copies): 218 -> 190 us at 32768 tokens x 40 heads x 128.  Everything else is loaded into registers,
+  // kBatch heads at a time (fp32 through shared memory took 179 instead of 138 us at 16384 tokens x 32 heads x 80).
+  constexpr bool kAhead = sizeof(T) == 2 && V == 8;
+  constexpr int kBatch = sizeof(T) == 4 || V == 1 ? 1 : 2, kDepth = 4;
+  __shared__ uint4 ring[kAhead ? kDepth : 1][2][2][kAhead ? kRotThreads : 1];   // x, dy; the lane's two vectors
   __shared__ float red[kRotMaxDim];
   const int which = (int)blockIdx.x < p.blocks0 ? 0 : 1;
   const int block = which == 0 ? blockIdx.x : blockIdx.x - p.blocks0;
@@ -430,10 +485,26 @@ __global__ void __launch_bounds__(kRotThreads, 4) qk_norm_rotary_bwd_kernel(cons
     const T* g = static_cast<const T*>(pg.p) + b * pg.sb + l * pg.st + first * pg.sh;
     T* y = static_cast<T*>(py.p) + b * py.sb + l * py.st + first * py.sh;
     typename View::Head raw_x[kBatch], raw_g[kBatch];
+    const auto ahead = [&](int slot, int k) {              // starts the copies of the k-th head from `first` on
+      if constexpr (kAhead) {
+        copy_ahead(&ring[slot][0][0][threadIdx.x], x + k * px.sh + view.ea[0]);
+        copy_ahead(&ring[slot][0][1][threadIdx.x], x + k * px.sh + view.eb[0]);
+        copy_ahead(&ring[slot][1][0][threadIdx.x], g + k * pg.sh + view.ea[0]);
+        copy_ahead(&ring[slot][1][1][threadIdx.x], g + k * pg.sh + view.eb[0]);
+      }
+    };
+    if constexpr (kAhead) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      view.load(x + min(k, last - 1 - first) * px.sh, raw_x[k]);
-      view.load(g + min(k, last - 1 - first) * pg.sh, raw_g[k]);
+      for (int k = 0; k < kDepth; ++k) {
+        if (first + k < last) ahead(k, k);
+        copy_ahead_commit();
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        view.load(x + min(k, last - 1 - first) * px.sh, raw_x[k]);
+        view.load(g + min(k, last - 1 - first) * pg.sh, raw_g[k]);
+      }
     }
     P c[N], sn[N];
     {
@@ -445,58 +516,71 @@ __global__ void __launch_bounds__(kRotThreads, 4) qk_norm_rotary_bwd_kernel(cons
         sn[j] = P::of(sf + j * View::W);
       }
     }
-    for (int h = first; h < last; h += kBatch) {
+    // one head, its vectors in registers
+    const auto work = [&](const typename View::Head& hx, const typename View::Head& hg, T* out) {
+      P xa[N], xb[N], ga[N], gb[N];
+      view.expand(hx, xa, xb);
+      view.expand(hg, ga, gb);
+      const float r = rsqrtf(group_sum(view.sum_of_products(xa, xa, xb, xb), p.group) * p.inv_dim + p.eps);
+      // t = r R(-angle) dy;  dw += t x;  u = t w;  dx = u - x r^2 mean(u x)
+      const P rr = P::all(r), minus = P::all(-1.f);
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (h + k < last) {                               // warp-uniform
-          P xa[N], xb[N], ga[N], gb[N];
-          view.expand(raw_x[k], xa, xb);
-          view.expand(raw_g[k], ga, gb);
-          const float r = rsqrtf(group_sum(view.sum_of_products(xa, xa, xb, xb), p.group) * p.inv_dim + p.eps);
-          // t = r R(-angle) dy;  dw += t x;  u = t w;  dx = u - x r^2 mean(u x)
-          const P rr = P::all(r), minus = P::all(-1.f);
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            if (view.turns[View::slot(j)]) {
-              const P ta = fma(mul(gb[j], minus), sn[j], mul(ga[j], c[j]));
-              gb[j] = fma(gb[j], c[j], mul(ga[j], sn[j]));
-              ga[j] = ta;
-            }
-            ga[j] = mul(ga[j], rr);
-            gb[j] = mul(gb[j], rr);
-            if (live) {                                   // a group behind the last token repeats it and adds nothing
-              dwa[j] = fma(ga[j], xa[j], dwa[j]);
-              dwb[j] = fma(gb[j], xb[j], dwb[j]);
-            }
-          }
-          {
-            P wa[N], wb[N];
-            view.load_weight(ws, wa, wb);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-              ga[j] = mul(ga[j], wa[j]);
-              gb[j] = mul(gb[j], wb[j]);
-            }
-          }
-          const float dot = group_sum(view.sum_of_products(ga, xa, gb, xb), p.group) * p.inv_dim;
-          const P f = P::all(-r * r * dot);
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            ga[j] = fma(xa[j], f, ga[j]);
-            gb[j] = fma(xb[j], f, gb[j]);
-          }
-          if (live) view.store(y + k * py.sh, ga, gb);
+      for (int j = 0; j < N; ++j) {
+        if (view.turns[View::slot(j)]) {
+          const P ta = fma(mul(gb[j], minus), sn[j], mul(ga[j], c[j]));
+          gb[j] = fma(gb[j], c[j], mul(ga[j], sn[j]));
+          ga[j] = ta;
+        }
+        ga[j] = mul(ga[j], rr);
+        gb[j] = mul(gb[j], rr);
+        if (live) {                                   // a group behind the last token repeats it and adds nothing
+          dwa[j] = fma(ga[j], xa[j], dwa[j]);
+          dwb[j] = fma(gb[j], xb[j], dwb[j]);
         }
       }
-      x += kBatch * px.sh;
-      g += kBatch * pg.sh;
-      y += kBatch * py.sh;
-      if (h + kBatch < last) {
+      {
+        P wa[N], wb[N];
+        view.load_weight(ws, wa, wb);
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-          view.load(x + min(k, last - 1 - h - kBatch) * px.sh, raw_x[k]);
-          view.load(g + min(k, last - 1 - h - kBatch) * pg.sh, raw_g[k]);
+        for (int j = 0; j < N; ++j) {
+          ga[j] = mul(ga[j], wa[j]);
+          gb[j] = mul(gb[j], wb[j]);
+        }
       }
+      const float dot = group_sum(view.sum_of_products(ga, xa, gb, xb), p.group) * p.inv_dim;
+      const P f = P::all(-r * r * dot);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        ga[j] = fma(xa[j], f, ga[j]);
+        gb[j] = fma(xb[j], f, gb[j]);
+      }
+      if (live) view.store(out, ga, gb);
+    };
+    if constexpr (kAhead) {
+      for (int h = first; h < last; ++h) {
+        const int slot = (h - first) & (kDepth - 1);
+        copy_ahead_wait<kDepth - 1>();
+        view.from_shared(ring[slot][0][0][threadIdx.x], ring[slot][0][1][threadIdx.x], raw_x[0]);
+        view.from_shared(ring[slot][1][0][threadIdx.x], ring[slot][1][1][threadIdx.x], raw_g[0]);
+        work(raw_x[0], raw_g[0], y + (h - first) * py.sh);
+        if (h + kDepth < last) ahead(slot, h - first + kDepth);
+        copy_ahead_commit();
+      }
+    } else {
+      for (int h = first; h < last; h += kBatch) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (h + k < last) work(raw_x[k], raw_g[k], y + k * py.sh);      // warp-uniform
+        x += kBatch * px.sh;
+        g += kBatch * pg.sh;
+        y += kBatch * py.sh;
+        if (h + kBatch < last) {
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            view.load(x + min(k, last - 1 - h - kBatch) * px.sh, raw_x[k]);
+            view.load(g + min(k, last - 1 - h - kBatch) * pg.sh, raw_g[k]);
+          }
+        }
       }
     }
   }

@@ -16,7 +16,7 @@
 // A head is held by a group of 1 to 32 lanes, up to eight pairs (two 16-byte vectors of bf16) a lane, so the
 // norm is a shuffle reduction inside the group and every element is read and written once:
 // HBM-bound (forward 4 bytes per bf16 element, norm backward 6).  Measured (B200, copy bandwidth 6.57 TB/s):
-// 65536 tokens x 40 heads x 128 bf16 rotation 204 us, 6.58 TB/s; 32768 tokens with norms forward 113 us, 5.9 TB/s,
+// 65536 tokens x 40 heads x 128 bf16 rotation 204 us, 6.58 TB/s; 32768 tokens with norms forward 107 us, 6.3 TB/s,
 // backward 183 us, 5.5 TB/s (bound by the chain of two reductions per head at 16 warps per SM).
 //
 // A group walks heads of ONE token, queries and keys, with the cosines and sines of its pairs in registers: no

@@ -4,7 +4,8 @@
 Tolerances.  A bf16 result is rounded once: half a step is 2^-8 of the value.  Before that, in fp32:
 cosine and sine are off by less than 2^-22 (the angle's float rounding, sincospi's own last bits), the
 products and sum of a pair by 3 * 2^-24, so a rotation is off by at most 2^-21 (|a| + |b|), taken
-here as 2^-20 of the head's largest element.  The norm's mean of squares adds at most 21 roundings in a
+here as 2^-20 of the head's largest element.  For bf16 the hardware's sine and cosine are used, which are off by up to
+2^-21.2 and would allow 1.5 * 2^-20 where every error points one way; the tolerance stays at 2^-20.  The norm's mean of squares adds at most 21 roundings in a
 chain (16 elements a lane, five shuffles) and rsqrt two, 2^-19 in all, halved by the square root.  The
 input gradient combines three such terms: 2^-17 of the tensor's largest element.  A weight gradient
 is a sum of n products, each off by 2^-19, with a chain of at most n additions: (2^-19 + n 2^-24) of

@@ -75,8 +75,12 @@ class RotaryPositions(nn.Module):
 
     @property
     def table(self):
-        buffers = self._buffers
-        return buffers["turns"], buffers["axis"], len(self.sections), self.layout == "interleaved"
+        buffers = self._buffers     # a third of an attribute's time; a replica of the module has attributes only
+        try:
+            turns, axis = buffers["turns"], buffers["axis"]
+        except KeyError:
+            turns, axis = self.turns, self.axis
+        return turns, axis, len(self.sections), self.layout == "interleaved"
 
     def _check(self, x):
         if x.shape[-1] != self.head_dim:
@@ -116,7 +120,11 @@ class FusedQKNorm(nn.Module):
             raise ValueError(f"head_dim {q.shape[-1]} is not this module's {self.head_dim}")
         table = _NO_TABLE if self.rotary is None else self.rotary.table
         params = self._parameters
-        return tuple(_ext().qk_norm_call(q, k, params["q_weight"], params["k_weight"], positions, *table, self.eps))
+        try:
+            q_weight, k_weight = params["q_weight"], params["k_weight"]
+        except KeyError:            # parametrized, pruned or replicated: attributes that are no parameters
+            q_weight, k_weight = self.q_weight, self.k_weight
+        return tuple(_ext().qk_norm_call(q, k, q_weight, k_weight, positions, *table, self.eps))
 
     def extra_repr(self):
         return f"head_dim={self.head_dim}, eps={self.eps}"

@@ -340,3 +340,25 @@ def test_refusals_on_the_gpu():
         mod(x, x)
     with pytest.raises(ValueError):
         FusedQKNorm(64).cuda()(x, x, p)
+
+
+def test_parametrized_weights():
+    """A parametrized weight is used as parametrized, and its gradient goes through the parametrization."""
+    from custom import FusedQKNorm
+
+    class Twice(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    gen = torch.Generator().manual_seed(3)
+    q = torch.randn(2, 9, 3, 64, generator=gen).cuda()
+    plain, made = FusedQKNorm(64).cuda(), FusedQKNorm(64).cuda()
+    torch.nn.utils.parametrize.register_parametrization(made, "q_weight", Twice())
+    with torch.no_grad():
+        plain.q_weight.fill_(2.0)
+    want, got = plain(q, q), made(q, q)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    original = made.parametrizations.q_weight.original
+    dwant, = torch.autograd.grad(want[0].square().sum(), plain.q_weight)
+    dgot, = torch.autograd.grad(got[0].square().sum(), original)
+    assert torch.equal(2 * dwant, dgot)                  # a factor of two is exact

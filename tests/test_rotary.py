@@ -103,3 +103,22 @@ def test_model_options_without_a_gpu():
         AttentionBlock(64, 4, rotary=RotaryPositions(16, (8,)))
     with pytest.raises(NotImplementedError):
         rope(torch.rand(2, 1, 28, 28))
+
+
+def test_weights_and_tables_that_are_plain_attributes():
+    """A parametrized or replicated module holds its weights and tables outside its parameter and buffer
+    dictionaries: the call still finds them (and then refuses tensors that are not on a GPU)."""
+    norm = FusedQKNorm(8, rotary=RotaryPositions(8, (2, 2)))
+    q, pos = torch.zeros(3, 2, 8), torch.zeros(3, 2, dtype=torch.int64)
+
+    class Twice(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    torch.nn.utils.parametrize.register_parametrization(norm, "q_weight", Twice())
+    with pytest.raises(NotImplementedError):
+        norm(q, q, pos)
+    replica = RotaryPositions(8, (2, 2))._replicate_for_data_parallel()
+    replica._buffers = {}
+    replica.turns, replica.axis = norm.rotary.turns, norm.rotary.axis
+    assert replica.table[0] is norm.rotary.turns and replica.table[1:] == (norm.rotary.axis, 2, False)

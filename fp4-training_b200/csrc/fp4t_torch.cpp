@@ -6,14 +6,17 @@
 // computes: every result comes from the kernels of libfp4t.so, on torch's current stream of the tensors'
 // device, and nothing synchronises.
 #include <ATen/autocast_mode.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <array>
 #include <atomic>
+#include <unordered_set>
 
 #include "../../include/fp4t.h"
 
@@ -68,6 +71,35 @@ variable_list once(variable_list grads, const variable_list& out_grads) {
   for (auto& g : grads)
     if (g.defined()) g = marked[i++];
   return grads;
+}
+
+// A captured backward pass must not reach a leaf whose gradient accumulator belongs to the default stream, which it does
+// while an eager graph of that leaf lives: that stream would be made to wait for the capturing one, which CUDA
+// forbids; the capture is lost and the process can end with it.  Looked for along the edges that this pass takes,
+// once per node and capture.
+void refuse_eager_leaves(const Tensor& like) {
+  const c10::cuda::OptionalCUDAGuard guard(like.device());
+  const auto standard = c10::cuda::getDefaultCUDAStream(like.get_device());
+  if (c10::cuda::getCurrentCUDAStream(like.get_device()) == standard) return;          // it cannot be captured
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto start = torch::autograd::get_current_node();
+  std::vector<torch::autograd::Node*> open{start.get()};
+  std::unordered_set<torch::autograd::Node*> seen{start.get()};
+  while (!open.empty()) {
+    torch::autograd::Node* node = open.back();
+    open.pop_back();
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+      torch::autograd::Node* next = node->next_edge(i).function.get();
+      if (!next || !node->task_should_compute_output(i) || !seen.insert(next).second) continue;
+      if (dynamic_cast<torch::autograd::AccumulateGrad*>(next)) {
+        const auto stream = next->stream();
+        TORCH_CHECK(!stream.has_value() || *stream != standard.unwrap(),
+                    "a backward pass is captured while an eager graph of the same leaves, built on the default stream, is alive: drop the eager "
+                    "graph's results first, or build it on another stream");
+      }
+      open.push_back(next);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ rotary positions, query / key norms
@@ -242,6 +274,7 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
     const auto saved = ctx->get_saved_variables();
     const int64_t layout = ctx->saved_data["layout"].toInt();
+    refuse_eager_leaves(saved[0]);
     // a rotation's transpose is the rotation back
     Heads dx = rotate(dy, Table{saved[0], saved[1], saved[2], layout / 2, (layout & 1) != 0}, true);
     return once({dx.t[0], dx.t[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, dy);
@@ -261,6 +294,7 @@ struct QKNormFn : public torch::autograd::Function<QKNormFn> {
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
     const auto s = ctx->get_saved_variables();
     const int64_t layout = ctx->saved_data["layout"].toInt();
+    refuse_eager_leaves(s[0]);
     auto [dx, dw] = norm_backward(dy, {s[0], s[1]}, {s[2], s[3]}, ctx->saved_data["eps"].toDouble(),
                                   Table{s[4], s[5], s[6], layout / 2, (layout & 1) != 0});
     for (int i = 0; i < 2; ++i) dw[i] = dw[i].to(s[2 + i].scalar_type());
@@ -421,6 +455,7 @@ struct XentFn : public torch::autograd::Function<XentFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const auto s = ctx->get_saved_variables();
     const auto args = ctx->saved_data["args"].toIntVector();
+    refuse_eager_leaves(s[0]);
     std::array<std::optional<at::ScalarType>, 3> want;
     if (ctx->needs_input_grad(0)) want[0] = (at::ScalarType)args[3];
     if (ctx->needs_input_grad(1)) want[1] = (at::ScalarType)args[4];

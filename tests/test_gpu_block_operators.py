@@ -202,3 +202,49 @@ def test_parameters_accumulate_like_any_others():
         (a.square().sum() + b.sum()).backward()
     once = torch.autograd.grad((lambda o: o[0].square().sum() + o[1].sum())(norm(q, q)), [norm.q_weight, norm.k_weight])
     assert torch.allclose(norm.q_weight.grad, 2 * once[0]) and torch.allclose(norm.k_weight.grad, 2 * once[1])
+
+
+def _leaves_and_calls():
+    """(leaves, call) of each operator: the call returns the tensor to differentiate."""
+    from custom import FusedQKNorm, RotaryPositions, linear_cross_entropy
+    gen = torch.Generator(device="cuda").manual_seed(11)
+
+    def rand(*shape):
+        return torch.randn(*shape, device="cuda", generator=gen).to(torch.bfloat16).requires_grad_()
+
+    rot = RotaryPositions(64, (16, 16)).cuda()
+    norm = FusedQKNorm(64, rotary=rot).cuda()
+    pos = torch.randint(0, 50, (40, 2), device="cuda", generator=gen)
+    q, k, x, h, w = rand(2, 40, 3, 64), rand(2, 40, 3, 64), rand(2, 40, 192), rand(100, 64), rand(300, 64)
+    t = torch.randint(0, 300, (100,), device="cuda", generator=gen)
+    return {
+        "rotary": ([q], lambda: rot(q, positions=pos)),
+        "norm": ([q, k, norm.q_weight], lambda: torch.cat(norm(q, k, pos))),
+        "norm_of_a_view": ([x], lambda: norm(x.view(2, 40, 3, 64), k.detach(), pos)[0]),
+        "loss": ([h, w], lambda: linear_cross_entropy(h, w, t)),
+    }
+
+
+@pytest.mark.parametrize("which", ["rotary", "norm", "norm_of_a_view", "loss"])
+def test_captured_backward_of_leaves_that_an_eager_graph_holds(which):
+    """While an eager graph of the same leaves lives on the default stream the captured backward is refused, before
+    anything that would spoil the capture; when it is gone the same call is captured and replays."""
+    leaves, call = _leaves_and_calls()[which]
+    eager = call()
+    seed = torch.ones_like(eager)
+    want = torch.autograd.grad(eager, leaves, seed, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+        with pytest.raises(RuntimeError, match="an eager graph of the same leaves"):
+            torch.autograd.grad(out, leaves, seed)
+    del out, graph
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, leaves, seed), want))
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call(), leaves, seed)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

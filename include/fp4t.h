@@ -540,7 +540,8 @@ FP4T_API int fp4t_qk_norm_rotary_backward(const fp4t_heads_t* dy, const fp4t_hea
  *   pass (of the counted tokens, in order); count [1]: how many were counted (fp32).
  * backward: any of dh [tokens, dim], dw [vocab, dim] and db [vocab] (contiguous, f32 or bf16; null: not
  *   wanted) from grad_loss ([1], or [tokens] with FP4T_XENT_NONE).  The logits' gradient is rounded to bf16,
- *   the operand type of the two products, which accumulate in fp32; db sums it before that rounding.
+ *   the operand type of the two products, which accumulate in fp32 (up to 64 tokens it is kept as a sum of two
+ *   bf16; a scalar grad_loss is applied behind the products); db sums it before that rounding.
  * Workspaces: 16-byte aligned, sizes from the two calls below (the backward one holds dl of one
  * piece, at most 512 MB or 4096 entries wide).  All results are reproducible.
  */
